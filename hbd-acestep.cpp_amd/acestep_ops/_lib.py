@@ -13,7 +13,7 @@ LIB_DIR = os.path.normpath(os.path.join(_PKG_DIR, "..", "lib"))
 LIB_PATH = os.environ.get("MI_OPS_LIB", os.path.join(LIB_DIR, "libmi_ops.so"))
 
 # enum mi_type (values equal enum ggml_type)
-F32, F16, Q8_0, I32, BF16 = 0, 1, 8, 26, 30
+F32, F16, Q4_0, Q8_0, I32, BF16 = 0, 1, 2, 8, 26, 30
 # enum mi_q8_0_rounding
 Q8_0_CPU_X86, Q8_0_REF = 0, 1
 

@@ -5,7 +5,7 @@ calls they replace; see include/mi_ops.h for the reference call sites).
 Operands are ``device.DTensor`` views: a shape (..., ne1, ne0) maps to the
 ggml view [ne0, ne1, ...] with byte strides taken from the element strides.
 Q8_0 tensors are uint8 tensors whose last axis holds whole 34-byte blocks
-(see ``Q8``). Every call is enqueued on ``stream`` (default: the null
+(see ``Q8``), Q4_0 tensors the same with 18-byte blocks (``Q4``). Every call is enqueued on ``stream`` (default: the null
 stream); errors raise ``MiError`` with the library's mi_status.
 """
 from __future__ import annotations
@@ -15,7 +15,7 @@ import struct
 from dataclasses import dataclass
 
 from . import _lib
-from ._lib import Q8_0, MiTensor
+from ._lib import Q4_0, Q8_0, MiTensor
 from .device import DTYPES, DTensor
 
 
@@ -33,6 +33,20 @@ class Q8:
         return tuple(self.data.shape[:-1]) + (self.ne0,)
 
 
+@dataclass
+class Q4:
+    """A Q4_0 tensor: ``data`` is a u8 DTensor with shape (..., n_blocks*18)."""
+    data: DTensor
+
+    @property
+    def ne0(self) -> int:
+        return self.data.shape[-1] // 18 * 32
+
+    @property
+    def shape(self):
+        return tuple(self.data.shape[:-1]) + (self.ne0,)
+
+
 _PACK = struct.Struct("=Qii4q4q").pack  # struct mi_tensor (a negative stride keeps its bits; the library refuses it)
 
 
@@ -41,17 +55,18 @@ def desc(t) -> MiTensor:
     passes here, and a short prompt's layer call waits for the host: one loop over the
     dimensions and one packed struct take 2.5 us where the view's own extent() and the
     ctypes fields set one by one took 5.4 (a 257-token prefill layer 179 -> 141 us)."""
-    if isinstance(t, Q8):
+    if isinstance(t, (Q8, Q4)):
         x = t.data
-        if x.dtype != "u8" or x.shape[-1] % 34 != 0 or x.strides[-1] != 1:
-            raise ValueError("Q8 data must be u8 (..., n_blocks*34) with contiguous blocks")
-        es, typ, q8 = 1, Q8_0, True
+        bsz, typ = (34, Q8_0) if isinstance(t, Q8) else (18, Q4_0)
+        if x.dtype != "u8" or x.shape[-1] % bsz != 0 or x.strides[-1] != 1:
+            raise ValueError(f"{type(t).__name__} data must be u8 (..., n_blocks*{bsz}) with contiguous blocks")
+        es = 1
     else:
         x = t
         es, _, typ = DTYPES[x.dtype]
         if typ is None:
             raise TypeError(f"dtype {x.dtype} is not an op operand type")
-        q8 = False
+        bsz = 0
     shape, strides = x.shape, x.strides
     if len(shape) > 4:
         raise ValueError("at most 4 dimensions")
@@ -80,8 +95,8 @@ def desc(t) -> MiTensor:
         ne.append(1)
         nb.append(es)
     blck = 1
-    if q8:
-        ne[0], nb[0], blck = ne[0] // 34 * 32, 34, 32  # nb[0] = block size
+    if bsz:
+        ne[0], nb[0], blck = ne[0] // bsz * 32, bsz, 32  # nb[0] = block size
     while len(ne) < 4:  # outer dims of size 1 continue contiguously
         nb.append(nb[-1] * ne[-1] // (blck if len(ne) == 1 else 1))
         ne.append(1)
@@ -197,7 +212,7 @@ def modulate(x, scale, shift, out=None, stream=None):
 
 
 def get_rows(table, ids, out=None, out_dtype="f32", err=None, stream=None):
-    """ggml_get_rows: table (n_rows, n) [or Q8], ids i32 (n_ids,) -> (n_ids, n)."""
+    """ggml_get_rows: table (n_rows, n) [or Q8, Q4], ids i32 (n_ids,) -> (n_ids, n)."""
     n = table.shape[-1]
     y = _out(out, (ids.shape[0], n), out_dtype)
     ep = ctypes.c_void_p(err.ptr) if err is not None else None
@@ -206,7 +221,7 @@ def get_rows(table, ids, out=None, out_dtype="f32", err=None, stream=None):
 
 
 def cpy(src, dst, rounding: int = _lib.Q8_0_CPU_X86, stream=None):
-    """ggml_cpy(src, dst) into a same-shape view (Q8 dst quantizes)."""
+    """ggml_cpy(src, dst) into a same-shape view (a Q8 or Q4 dst quantizes)."""
     _lib.call("mi_cpy_q8_0", _p(src), _p(dst), rounding, _s(stream))
     return dst
 

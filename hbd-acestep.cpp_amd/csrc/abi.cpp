@@ -68,7 +68,7 @@ int check(const mi_tensor * t, bool inner = true) {
             return MI_ERR_SHAPE;
         }
     }
-    if (t->type == MI_TYPE_Q8_0 && t->ne[0] % 32 != 0) {
+    if (is_block(t->type) && t->ne[0] % 32 != 0) {
         return MI_ERR_SHAPE;
     }
     // the row count, element count and byte extent must each fit in int64:
@@ -95,7 +95,7 @@ int check(const mi_tensor * t, bool inner = true) {
     if (nelements(*t) > 0 && !t->data) {
         return MI_ERR_NULL;
     }
-    const size_t al = t->type == MI_TYPE_Q8_0 ? 2 : (size_t) es;
+    const size_t al = is_block(t->type) ? 2 : (size_t) es;
     if (!aligned(t->data, al)) {
         return MI_ERR_ALIGN;
     }
@@ -527,7 +527,7 @@ int mi_get_rows(const mi_tensor * table, const mi_tensor * ids, const mi_tensor 
     MI_TRY(check(table));
     MI_TRY(check(ids, false));
     MI_TRY(check(y));
-    if (table->type != MI_TYPE_Q8_0 && !is_act(table->type)) {
+    if (!is_block(table->type) && !is_act(table->type)) {
         return MI_ERR_TYPE;
     }
     if (ids->type != MI_TYPE_I32 || (y->type != MI_TYPE_F32 && y->type != MI_TYPE_BF16)) {
@@ -562,7 +562,7 @@ static RowCopy plain_copy(const mi_tensor & src, const mi_tensor & dst) {
 int mi_cpy_q8_0(const mi_tensor * src, const mi_tensor * dst, int rounding, mi_stream stream) {
     MI_TRY(check_act(src));
     MI_TRY(check(dst));
-    if (dst->type != MI_TYPE_Q8_0 && !is_act(dst->type)) {
+    if (!is_block(dst->type) && !is_act(dst->type)) {
         return MI_ERR_TYPE;
     }
     if (!same_shape(*src, *dst)) {
@@ -583,7 +583,7 @@ static int kv_desc(const mi_tensor * x, const mi_tensor * cache, const mi_tensor
                    int32_t * d_err, RowCopy & r) {
     MI_TRY(check_act(x));
     MI_TRY(check(cache));
-    if (cache->type != MI_TYPE_Q8_0 && !is_act(cache->type)) {
+    if (!is_block(cache->type) && !is_act(cache->type)) {
         return MI_ERR_TYPE;
     }
     if (cache->ne[0] != x->ne[0] || cache->ne[2] != x->ne[1]) {
@@ -705,7 +705,7 @@ int mi_qk_norm_rope_kv_store(const mi_tensor * q, const mi_tensor * q_w, const m
     // [ne2 * ne3] order belongs to sequence t / T, T = tokens / B
     MI_TRY(check(k_cache));
     MI_TRY(check(v_cache));
-    if (k_cache->type != MI_TYPE_Q8_0 && !is_act(k_cache->type)) {
+    if (!is_block(k_cache->type) && !is_act(k_cache->type)) {
         return MI_ERR_TYPE;
     }
     if (!same_shape(*k_cache, *v_cache) || k_cache->type != v_cache->type || k_cache->nb[1] != v_cache->nb[1] ||

@@ -261,6 +261,39 @@ __device__ __forceinline__ float div127(float amax) {
     return __builtin_fmaf(r, C, q0);
 }
 
+// ---------------------------------------------------------------------------
+// Q4_0 block quantizer pieces. With m the element of the largest magnitude (the
+// first of equal ones): d = m / -8, id = d ? 1 / d : 0, q = min(15, floor(x id +
+// 8.5)), so m takes level 0 and zero level 8. Magnitudes are compared as bits: a
+// NaN is then larger than every number and makes the block's d a NaN, an
+// infinity makes d infinite, its own level 0 and the others' 8, (8 - 8) * inf = NaN.
+// ---------------------------------------------------------------------------
+template <int N> __device__ __forceinline__ void q4_top(const float * f, uint32_t & u, float & m) {
+    u = __float_as_uint(f[0]) & 0x7fffffffu;
+    m = f[0];
+#pragma unroll
+    for (int e = 1; e < N; ++e) {
+        const uint32_t v = __float_as_uint(f[e]) & 0x7fffffffu;
+        m                = v > u ? f[e] : m;
+        u                = v > u ? v : u;
+    }
+}
+
+// the levels of 4 elements, a byte each
+__device__ __forceinline__ uint32_t q4_levels4(const float * f, float id) {
+    uint32_t w = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float v = f[e] * id + 8.5f;
+        w |= (uint32_t) __builtin_amdgcn_fmed3f(v, 0.0f, 15.0f) << (8 * e);  // positive: the cast is the floor
+    }
+    return w;
+}
+
+__device__ __forceinline__ float q4_inv(float d) {
+    return d != 0.0f ? 1.0f / d : 0.0f;
+}
+
 // An optimization barrier on a register quad: its value is treated as changed,
 // so values derived from it before are recomputed after, not kept live.
 __device__ __forceinline__ void opaque(uint4 & v) {
@@ -444,13 +477,20 @@ inline int type_size(int t) {
             return 2;
         case MI_TYPE_Q8_0:
             return 34;
+        case MI_TYPE_Q4_0:
+            return 18;
         default:
             return 0;
     }
 }
 
+// block types: 32 elements a block, 2-byte aligned
+inline bool is_block(int t) {
+    return t == MI_TYPE_Q8_0 || t == MI_TYPE_Q4_0;
+}
+
 inline int blck_size(int t) {
-    return t == MI_TYPE_Q8_0 ? 32 : 1;
+    return is_block(t) ? 32 : 1;
 }
 
 inline bool is_act(int t) {

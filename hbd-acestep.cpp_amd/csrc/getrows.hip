@@ -273,6 +273,61 @@ __global__ void __launch_bounds__(256) k_get_rows_q8_0_flat(const GetRowsArgs a,
     }
 }
 
+// Q4_0 rows: y = (q - 8) * d, exact in fp32 (4 + 11 significant bits). Flat, as
+// above, but a thread makes 2 * OPS outputs from one load of OPS bytes: the low
+// nibbles are elements e .. e + OPS - 1 of a block's first half, the high ones
+// the same of its second half, so every byte is read once.
+template <int TO, int U>
+__global__ void __launch_bounds__(256) k_get_rows_q4_0_flat(const GetRowsArgs a, FastDiv per_row, uint32_t nchunks) {
+    constexpr int  EO  = TT<TO>::ES;
+    constexpr int  OPS = 16 / EO;   // bytes of quants per thread, outputs per store
+    constexpr int  CPB = 16 / OPS;  // threads per block
+    const uint32_t c0  = blockIdx.x * (256 * U) + threadIdx.x;
+    uint32_t       i[U];
+    int            o[U];
+    int64_t        r[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const uint32_t c = c0 + 256 * u < nchunks ? c0 + 256 * u : nchunks - 1;  // clamped: loads stay in bounds
+        i[u]             = per_row.div(c);
+        o[u]             = (int) (c - i[u] * per_row.d);
+        r[u]             = a.ids[(int64_t) i[u] * a.ids_stride];
+    }
+    uint16_t dh[U], q[U][OPS / 2];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const bool       ok = r[u] >= 0 && r[u] < a.n_rows;
+        const char *     bp = a.table + (ok ? r[u] : 0) * a.tnb1 + (int64_t) (o[u] / CPB) * 18;
+        const uint16_t * qp = (const uint16_t *) (bp + 2 + (o[u] % CPB) * OPS);
+        dh[u]               = *(const uint16_t *) bp;
+#pragma unroll
+        for (int h = 0; h < OPS / 2; ++h) {
+            q[u][h] = qp[h];
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        if (c0 + 256 * u >= nchunks) {
+            break;
+        }
+        const bool bad = r[u] < 0 || r[u] >= a.n_rows;
+        if (bad && o[u] == 0 && a.d_err) {
+            atomicAdd(a.d_err, 1);
+        }
+        const float d = (float) __builtin_bit_cast(_Float16, dh[u]);
+        float       lo[OPS], hi[OPS];
+#pragma unroll
+        for (int k = 0; k < OPS; ++k) {
+            const uint32_t b = (uint32_t) q[u][k / 2] >> (8 * (k % 2));
+            lo[k]            = bad ? 0.0f : (float) ((int32_t) (b & 15u) - 8) * d;
+            hi[k]            = bad ? 0.0f : (float) ((int32_t) (b >> 4 & 15u) - 8) * d;
+        }
+        char * yp = a.y + (int64_t) i[u] * a.ynb1 + (int64_t) ((o[u] / CPB) * 32 + (o[u] % CPB) * OPS) * EO;
+        store_vec<TO, OPS>(yp, lo);
+        store_vec<TO, OPS>(yp + 16 * EO, hi);
+    }
+}
+
 #ifndef MI_GR_FLAT_U
 #define MI_GR_FLAT_U 4  // output chunks per thread in the flat kernel
 #endif
@@ -299,6 +354,13 @@ __global__ void __launch_bounds__(256) k_get_rows_generic(const GetRowsArgs a, i
                         const char *   bp = row + (size_t) (j >> 5) * 34;
                         const uint16_t dh = *(const uint16_t *) bp;
                         v = (float) (int8_t) bp[2 + (j & 31)] * (float) __builtin_bit_cast(_Float16, dh);
+                        break;
+                    }
+                    case MI_TYPE_Q4_0: {
+                        const char *   bp = row + (size_t) (j >> 5) * 18;
+                        const uint16_t dh = *(const uint16_t *) bp;
+                        const uint32_t q  = (uint32_t) (uint8_t) bp[2 + (j & 15)] >> (j & 16 ? 4 : 0) & 15u;
+                        v = (float) ((int32_t) q - 8) * (float) __builtin_bit_cast(_Float16, dh);
                         break;
                     }
                     case MI_TYPE_F32:
@@ -356,6 +418,18 @@ static int launch_to(const GetRowsArgs & a, int ttype, bool fast, bool lds, hipS
                 }
                 return MI_OK;
             }
+            case MI_TYPE_Q4_0: {
+                constexpr int      OPS     = 16 / TT<TO>::ES;
+                constexpr uint32_t per_wg  = 256 * MI_GR_FLAT_U / 2;  // half as many: a chunk is two stores
+                const uint64_t     nchunks = (uint64_t) a.n_ids * (uint64_t) (a.n / (2 * OPS));
+                if (a.n_rows > 0 && nchunks < (1ull << 31)) {  // an invalid id loads from row 0
+                    MI_LAUNCH((k_get_rows_q4_0_flat<TO, MI_GR_FLAT_U / 2>),
+                                       dim3((uint32_t) ((nchunks + per_wg - 1) / per_wg)), dim3(256), 0, s, a,
+                                       FastDiv((uint32_t) (a.n / (2 * OPS))), (uint32_t) nchunks);
+                    return MI_OK;
+                }
+                break;
+            }
             case MI_TYPE_F32:
                 MI_LAUNCH((k_get_rows_vec<MI_TYPE_F32, TO>), dim3(grid), dim3(256), 0, s, a);
                 return MI_OK;
@@ -396,6 +470,9 @@ int launch_get_rows(const mi_tensor & table, const int32_t * ids, int64_t n_ids,
                (a.ynb1 % 16 == 0) && (8 * es_out) % 16 == 0;
         // whole rows through LDS: rows of 16-byte multiples (ne0 % 256 == 0), 16-byte aligned
         lds = fast && a.n % 256 == 0 && a.n <= 8192 && aligned(table.data, 16) && a.tnb1 % 16 == 0;
+    } else if (table.type == MI_TYPE_Q4_0) {
+        // whole blocks; 16-bit aligned quants; output 16-byte stores
+        fast = aligned(table.data, 2) && a.tnb1 % 2 == 0 && aligned(y.data, 16) && a.ynb1 % 16 == 0;
     } else {
         const int VI = 16 / type_size(table.type);
         fast         = a.n % VI == 0 && aligned(table.data, 16) && a.tnb1 % 16 == 0 && aligned(y.data, 16) &&

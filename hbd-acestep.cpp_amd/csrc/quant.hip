@@ -1,4 +1,4 @@
-// quant.hip -- ggml_cpy into KV caches: F32/BF16/F16 -> Q8_0 / F16 / BF16 / F32,
+// quant.hip -- ggml_cpy into KV caches: F32/BF16/F16 -> Q8_0 / Q4_0 / F16 / BF16 / F32,
 // as a plain strided copy (mi_cpy) or as a batched scatter at per-sequence
 // slot offsets (mi_kv_store).
 //
@@ -284,6 +284,95 @@ __global__ void __launch_bounds__(256) k_row_q8_lds(const RowCopy K, const RowCo
     }
 }
 
+// Q4_0 destinations, staged as k_row_q8_lds: a wave's tile of 32 consecutive
+// blocks comes into LDS by lane-contiguous 16-byte loads, then a lane pair
+// quantizes each block, the first lane elements 0-15 and the second 16-31. Byte j
+// holds the levels of elements j and j + 16, so the lanes exchange their levels
+// (one DPP swap) and store 8 of the 16 bytes each.
+template <int TI>
+__global__ void __launch_bounds__(256) k_row_q4_lds(const RowCopy K, const RowCopy V, uint32_t nbk, uint32_t nbv,
+                                                    uint32_t wg_k, uint32_t nbpr, FastDiv dnbpr) {
+    constexpr int  EI  = TT<TI>::ES;
+    constexpr int  VEC = TT<TI>::VEC;    // elements per 16-byte chunk
+    constexpr int  CPB = 32 / VEC;       // chunks per block
+    constexpr int  CPL = 32 * CPB / 64;  // chunks per lane per tile (F32: 4, BF16/F16: 2)
+    __shared__ uint4 tile[4][32 * CPB];
+    const int      lane = threadIdx.x & 63;
+    const uint32_t wv   = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const bool      isv   = blockIdx.x >= wg_k;  // workgroups [0, wg_k) store K, the rest V
+    const RowCopy & R     = isv ? V : K;
+    const uint32_t  total = isv ? nbv : nbk;
+    const uint32_t  t0    = ((isv ? blockIdx.x - wg_k : blockIdx.x) * 4 + wv) * 32;  // first block of the tile
+    if (t0 >= total) {
+        return;  // whole wave
+    }
+    uint4 v[CPL];
+#pragma unroll
+    for (int k = 0; k < CPL; ++k) {  // blocks past the end load the last one again and are never read
+        const int      c  = lane + 64 * k;
+        const uint32_t gt = t0 + c / CPB;
+        const uint32_t g  = gt < total ? gt : total - 1;
+        const uint32_t w  = dnbpr.div(g);
+        const uint32_t bi = g - w * nbpr;
+        v[k]              = ld16(src_ptr(R, w) + (size_t) (bi * 32 + (c % CPB) * VEC) * EI);
+    }
+    const int      j   = lane >> 1;
+    const int      sub = lane & 1;
+    const uint32_t g   = t0 + j;
+    const uint32_t gc  = g < total ? g : total - 1;
+    const uint32_t w   = dnbpr.div(gc);
+    const uint32_t bi  = gc - w * nbpr;
+    const char *   srow;
+    char *         drow;
+    bool           bad;
+    row_ptrs(R, w, srow, drow, bad);
+#pragma unroll
+    for (int k = 0; k < CPL; ++k) {
+        tile[wv][lane + 64 * k] = v[k];
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    if (g >= total) {
+        return;  // whole pairs; nothing below synchronizes
+    }
+    if (bad) {
+        if (sub == 0 && bi == 0 && R.d_err) {
+            atomicAdd(R.d_err, 1);
+        }
+        return;
+    }
+    float f[16];
+#pragma unroll
+    for (int k = 0; k < 16 / VEC; ++k) {
+        unpack16<TI>(tile[wv][j * CPB + sub * (CPB / 2) + k], f + VEC * k);
+    }
+    uint32_t u;
+    float    m;
+    q4_top<16>(f, u, m);
+    const float    mo = dpp_f<0xB1>(m);
+    const uint32_t uo = __float_as_uint(mo) & 0x7fffffffu;
+    m                 = uo > u || (uo == u && sub) ? mo : m;  // of equal magnitudes the first lane's
+    const float d     = m * -0.125f;
+    const float id    = q4_inv(d);
+    uint32_t    own[4], oth[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        own[q] = q4_levels4(f + 4 * q, id);
+        oth[q] = (uint32_t) __builtin_amdgcn_update_dpp(0, (int) own[q], 0xB1, 0xf, 0xf, false);
+    }
+    const uint32_t b0 = sub ? oth[2] | own[2] << 4 : own[0] | oth[0] << 4;
+    const uint32_t b1 = sub ? oth[3] | own[3] << 4 : own[1] | oth[1] << 4;
+    char *         bp = drow + (size_t) bi * 18;
+    uint16_t *     qp = (uint16_t *) (bp + 2 + sub * 8);  // 2-byte aligned
+    qp[0]             = (uint16_t) (b0 & 0xffffu);
+    qp[1]             = (uint16_t) (b0 >> 16);
+    qp[2]             = (uint16_t) (b1 & 0xffffu);
+    qp[3]             = (uint16_t) (b1 >> 16);
+    if (sub == 0) {
+        *(uint16_t *) bp = f32_to_f16_bits(d);
+    }
+}
+
 // F32 / F16 / BF16 destinations: 4 lanes per 32 elements, 8 per lane.
 template <int TI, int TO>
 __global__ void __launch_bounds__(256) k_row_copy(const RowCopy K, const RowCopy V, uint32_t nbk, uint32_t total,
@@ -365,6 +454,27 @@ __global__ void __launch_bounds__(256) k_row_copy_generic(const RowCopy K, const
             const uint16_t dh = f32_to_f16_bits(d);
             bp[0]             = (char) (dh & 0xff);
             bp[1]             = (char) (dh >> 8);
+        } else if constexpr (TO == MI_TYPE_Q4_0) {
+            float x[32];
+            for (int e = 0; e < 32; ++e) {
+                x[e] = load_elem<TI>(srow + (size_t) (c * 32 + e) * EI);
+            }
+            uint32_t u;
+            float    m;
+            q4_top<32>(x, u, m);
+            const float d  = m * -0.125f;
+            const float id = q4_inv(d);
+            char *      bp = drow + (size_t) c * 18;
+            for (int e = 0; e < 16; e += 4) {
+                const uint32_t w = q4_levels4(x + e, id) | q4_levels4(x + 16 + e, id) << 4;
+                bp[2 + e]        = (char) (w & 0xff);
+                bp[3 + e]        = (char) (w >> 8 & 0xff);
+                bp[4 + e]        = (char) (w >> 16 & 0xff);
+                bp[5 + e]        = (char) (w >> 24);
+            }
+            const uint16_t dh = f32_to_f16_bits(d);
+            bp[0]             = (char) (dh & 0xff);
+            bp[1]             = (char) (dh >> 8);
         } else {
             const float v = load_elem<TI>(srow + (size_t) c * EI);
             store_elem<TO>(drow + (size_t) c * TT<TO>::ES, v);
@@ -391,6 +501,11 @@ static int launch_k(const RowCopy & K, const RowCopy * V, bool fast, hipStream_t
             MI_LAUNCH((k_row_q8<TI, ROUND>), dim3(grid), dim3(256), 0, s, K, Vr, nbk, total, nbpr,
                                FastDiv(nbpr));
 #endif
+        } else if constexpr (TO == MI_TYPE_Q4_0) {
+            const uint32_t nbv  = total - nbk;
+            const uint32_t wg_k = (nbk + 127) / 128;  // 4 waves x 32 blocks per workgroup
+            MI_LAUNCH((k_row_q4_lds<TI>), dim3(wg_k + (nbv + 127) / 128), dim3(256), 0, s, K, Vr, nbk, nbv, wg_k,
+                               nbpr, FastDiv(nbpr));
         } else {
             const uint32_t grid = (total * 4 + 255) / 256;
             MI_LAUNCH((k_row_copy<TI, TO>), dim3(grid), dim3(256), 0, s, K, Vr, nbk, total, nbpr,
@@ -398,7 +513,7 @@ static int launch_k(const RowCopy & K, const RowCopy * V, bool fast, hipStream_t
         }
         return MI_OK;
     }
-    const int      per_row = TO == MI_TYPE_Q8_0 ? K.ne0 / 32 : K.ne0;
+    const int      per_row = is_block(TO) ? K.ne0 / 32 : K.ne0;
     const uint64_t nk      = (uint64_t) K.rows * per_row;
     const uint64_t total   = nk + (V ? (uint64_t) V->rows * per_row : 0);
     uint64_t       grid    = (total + 255) / 256;
@@ -422,6 +537,8 @@ static int launch_ti(const RowCopy & K, const RowCopy * V, int tout, int roundin
     switch (tout) {
         case MI_TYPE_Q8_0:
             return launch_r<TI, MI_TYPE_Q8_0>(K, V, rounding, fast, s);
+        case MI_TYPE_Q4_0:
+            return launch_r<TI, MI_TYPE_Q4_0>(K, V, rounding, fast, s);
         case MI_TYPE_F32:
             return launch_r<TI, MI_TYPE_F32>(K, V, rounding, fast, s);
         case MI_TYPE_BF16:
@@ -437,7 +554,7 @@ static bool row_aligned(const RowCopy & R, int tin, int tout) {
     if (!aligned(R.src, sa) || R.sr.s1 % sa || R.sr.s2 % sa || R.sr.s3 % sa) {
         return false;
     }
-    if (tout == MI_TYPE_Q8_0) {  // 16-bit stores into 34-byte blocks
+    if (is_block(tout)) {  // 16-bit stores into 34- or 18-byte blocks
         return aligned(R.dst, 2) && (R.kv ? (R.cnb1 % 2 == 0 && R.cnb2 % 2 == 0 && R.cnb3 % 2 == 0)
                                           : (R.dr.s1 % 2 == 0 && R.dr.s2 % 2 == 0 && R.dr.s3 % 2 == 0));
     }
@@ -452,7 +569,7 @@ int launch_row_copy(const RowCopy & K, const RowCopy * V, int tin, int tout, int
     }
     bool fast = K.ne0 % 32 == 0 && row_aligned(K, tin, tout) && (!V || row_aligned(*V, tin, tout));
     fast      = fast && (uint64_t) (K.rows + (V ? V->rows : 0)) * (K.ne0 / 32) * 4 < (1ull << 31) &&
-           (tout != MI_TYPE_Q8_0 || K.ne0 % 32 == 0);
+           (!is_block(tout) || K.ne0 % 32 == 0);
     switch (tin) {
         case MI_TYPE_F32:
             return launch_ti<MI_TYPE_F32>(K, V, tout, rounding, fast, s);

@@ -540,7 +540,9 @@ int launch_heads(HeadArgs & a, int tin, int tout, hipStream_t s) {
 // type before the cache cast, as the separate ops store and reload it; V is
 // clamped first when asked (qwen3-lm.h:674-677). Q8_0 caches: a 32-element
 // block spans 32 / VI lanes of a row; they share the block's amax (DPP max),
-// each writes its VI quants (2-byte aligned) and the first the fp16 scale.
+// each writes its VI quants (2-byte aligned) and the first the fp16 scale. Q4_0:
+// the same lanes, byte j with the levels of elements j and j + 16, so the lanes of a
+// block's first half fetch the second half's levels and store.
 namespace mi {
 
 template <int TI, int TC, int D, int ROUND, bool TOCACHE = true>
@@ -748,6 +750,49 @@ __global__ void __launch_bounds__(256) k_heads_kv(const HeadArgs a, const HeadKV
                 }
             }
         }
+    } else if constexpr (TC == MI_TYPE_Q4_0) {
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+            const float * f  = part ? x1 : x0;
+            const int     el = (part ? HALF : 0) + j * VI;  // first element of this lane's chunk
+            const int     at = j % LPB;                     // this lane's place in its block
+            uint32_t      u;
+            float         m;
+            q4_top<VI>(f, u, m);
+            // the block's largest magnitude, then the sign of the first element that has it
+            uint32_t um = u;
+#pragma unroll
+            for (int o = 1; o < LPB; o *= 2) {
+                const uint32_t v = (uint32_t) __shfl_xor((int) um, o, 64);
+                um               = v > um ? v : um;
+            }
+            uint32_t first = u == um ? (uint32_t) at * 2 + (__float_as_uint(m) >> 31) : 64u;
+#pragma unroll
+            for (int o = 1; o < LPB; o *= 2) {
+                const uint32_t v = (uint32_t) __shfl_xor((int) first, o, 64);
+                first            = v < first ? v : first;
+            }
+            const float d  = __uint_as_float(um | first << 31) * -0.125f;
+            const float id = q4_inv(d);
+            uint32_t    w[VI / 4];
+#pragma unroll
+            for (int q = 0; q < VI / 4; ++q) {
+                w[q] = q4_levels4(f + 4 * q, id);
+                w[q] |= (uint32_t) __shfl_xor((int) w[q], LPB / 2, 64) << 4;  // element + 16's (first half of the lanes)
+            }
+            if (ok && at < LPB / 2) {
+                char *     bp = crow + (size_t) (el / 32) * 18;
+                uint16_t * qp = (uint16_t *) (bp + 2 + el % 32);
+#pragma unroll
+                for (int q = 0; q < VI / 4; ++q) {
+                    qp[2 * q]     = (uint16_t) (w[q] & 0xffffu);
+                    qp[2 * q + 1] = (uint16_t) (w[q] >> 16);
+                }
+                if (at == 0) {
+                    *(uint16_t *) bp = f32_to_f16_bits(d);
+                }
+            }
+        }
     } else {
         constexpr int EC = TT<TC>::ES;
         if (ok) {
@@ -800,6 +845,8 @@ static int launch_kv_c(const HeadArgs & a, const HeadKV & kv, int tcache, int ro
     switch (tcache) {
         case MI_TYPE_Q8_0:
             return launch_kv_t<TI, MI_TYPE_Q8_0>(a, kv, rounding, s);
+        case MI_TYPE_Q4_0:
+            return launch_kv_t<TI, MI_TYPE_Q4_0>(a, kv, rounding, s);
         case MI_TYPE_F16:
             return launch_kv_t<TI, MI_TYPE_F16>(a, kv, rounding, s);
         case MI_TYPE_BF16:
@@ -827,8 +874,8 @@ int launch_heads_kv(HeadArgs & a, const HeadKV & kv, int tin, int tcache, int ro
     fast = fast && aligned(Q.y, 16) && Q.ys1 % 16 == 0 && Q.ys2 % 16 == 0 && Q.ys3 % 16 == 0;
     fast = fast && aligned(kv.v, 16) && kv.vs1 % 16 == 0 && kv.vs2 % 16 == 0 && kv.vs3 % 16 == 0;
     // cache rows: 16-byte vectors for F16/BF16/F32 (half a row for F32 of D = 64 is 128 bytes);
-    // Q8_0 rows are 2-byte aligned blocks
-    const size_t ca = tcache == MI_TYPE_Q8_0 ? 2 : 16;
+    // Q8_0 and Q4_0 rows are 2-byte aligned blocks
+    const size_t ca = is_block(tcache) ? 2 : 16;
     fast = fast && aligned(kv.kc, ca) && aligned(kv.vc, ca) && kv.cnb1 % ca == 0 && kv.cnb2 % ca == 0 &&
            kv.cnb3 % ca == 0;
     if (!fast) {

@@ -15,6 +15,9 @@
  *
  * Q8_0 tensors follow ggml: ne[0] counts elements (a multiple of 32), nb[0]
  * is the 34-byte block size, a block is { fp16 d; int8 qs[32] }.
+ * Q4_0 tensors (4-bit KV caches, tables) likewise: an 18-byte block is { fp16 d;
+ * uint8 qs[16] }, byte j holding the level of element j in its low and of
+ * element j + 16 in its high nibble; a level q stands for (q - 8) * d.
  *
  * Activation tensors may be F32 or BF16 (BF16 is computed as bf16 -> f32,
  * the fp32 op chain, f32 -> bf16 round-to-nearest-even at the output).
@@ -35,6 +38,7 @@ extern "C" {
 enum mi_type {
     MI_TYPE_F32  = 0,
     MI_TYPE_F16  = 1,
+    MI_TYPE_Q4_0 = 2,
     MI_TYPE_Q8_0 = 8,
     MI_TYPE_I32  = 26,
     MI_TYPE_BF16 = 30,
@@ -164,7 +168,7 @@ int mi_gated_add(const mi_tensor * residual, const mi_tensor * x, const mi_tenso
 int mi_modulate(const mi_tensor * x, const mi_tensor * scale, const mi_tensor * shift, const mi_tensor * y,
                 mi_stream stream);
 
-/* ggml_get_rows(table, ids): table [n, n_rows] Q8_0/F16/BF16/F32, ids I32
+/* ggml_get_rows(table, ids): table [n, n_rows] Q8_0/Q4_0/F16/BF16/F32, ids I32
  * [n_ids] -> y [n, n_ids] F32 (or BF16). Replaces the embedding lookups at
  * qwen3-enc.h:390, 465, qwen3-lm.h:464, 626. ids may be strided (nb[0] any
  * multiple of 4, as ggml reads src1 through nb10). An id outside [0, n_rows)
@@ -173,14 +177,19 @@ int mi_modulate(const mi_tensor * x, const mi_tensor * scale, const mi_tensor * 
 int mi_get_rows(const mi_tensor * table, const mi_tensor * ids, const mi_tensor * y, int32_t * d_err,
                 mi_stream stream);
 
-/* ggml_cpy(src, dst): src F32/BF16/F16, dst F32/BF16/F16/Q8_0 view of the
- * same shape (any strides; Q8_0 dst rows are whole blocks). Q8_0 uses the
- * ggml-cpu x86 from_float rounding (MI_Q8_0_CPU_X86). Replaces the KV-cache
+/* ggml_cpy(src, dst): src F32/BF16/F16, dst F32/BF16/F16/Q8_0/Q4_0 view of the
+ * same shape (any strides; Q8_0 and Q4_0 dst rows are whole blocks). Q8_0 uses
+ * the ggml-cpu x86 from_float rounding (MI_Q8_0_CPU_X86). Replaces the KV-cache
  * writes at qwen3-lm.h:405-406, 701-702, songgen-lelm-gen.h:264-265,
- * 559-560. */
+ * 559-560.
+ * Q4_0: with m the block's element of the largest magnitude (the first of
+ * equal ones), d = m / -8, id = d != 0 ? 1 / d : 0, each level is
+ * min(15, floor(x * id + 8.5)) in fp32 and d is stored as fp16. A block with a
+ * NaN or an infinity has no finite value when it is read back. */
 int mi_cpy(const mi_tensor * src, const mi_tensor * dst, mi_stream stream);
 
-/* mi_cpy with an explicit Q8_0 rounding variant (enum mi_q8_0_rounding). */
+/* mi_cpy with an explicit Q8_0 rounding variant (enum mi_q8_0_rounding; other
+ * types ignore it). */
 int mi_cpy_q8_0(const mi_tensor * src, const mi_tensor * dst, int rounding, mi_stream stream);
 
 /* KV-cache store for a batch of sequences in one launch, replacing the N
@@ -188,7 +197,7 @@ int mi_cpy_q8_0(const mi_tensor * src, const mi_tensor * dst, int rounding, mi_s
  * (qwen3-lm.h:682-703) and the prefill cpy (qwen3-lm.h:396-406,
  * songgen-lelm-gen.h:254-265, 548-562).
  *   k, v:       [D, Nkv, T, B]  F32/BF16/F16 (v may be NULL)
- *   k/v_cache:  [D, max_seq, Nkv, n_sets] Q8_0/F16/BF16/F32
+ *   k/v_cache:  [D, max_seq, Nkv, n_sets] Q8_0/Q4_0/F16/BF16/F32
  *   pos0:       I32 [B]   first slot written for sequence b
  *   sets:       I32 [B] or NULL (set = b)
  * cache[:, pos0[b] + t, h, sets[b]] = k[:, h, t, b]. Out-of-range slots or
@@ -206,10 +215,10 @@ int mi_kv_store(const mi_tensor * k, const mi_tensor * k_cache, const mi_tensor 
  * not modified.
  *   q, q_out: [D, Nh, ne2, ne3]; k, v: [D, Nkv, ne2, ne3]; one activation type
  *   q_w, k_w: F32 [D] or both NULL (rope only); pos: I32 [ne2]
- *   k_cache, v_cache: [D, max_seq, Nkv, n_sets], one type (Q8_0/F16/BF16/F32)
+ *   k_cache, v_cache: [D, max_seq, Nkv, n_sets], one type (Q8_0/Q4_0/F16/BF16/F32)
  *   pos0, sets, rounding, d_err: as mi_kv_store
  * Needs D in {64, 128, 256} rotated whole (n_dims == D) and 16-byte aligned
- * q/k/v/q_out rows (2-byte for Q8_0 caches, 16-byte otherwise); other
+ * q/k/v/q_out rows (2-byte for Q8_0 and Q4_0 caches, 16-byte otherwise); other
  * layouts return MI_ERR_UNSUPPORTED (use the three calls). */
 int mi_qk_norm_rope_kv_store(const mi_tensor * q, const mi_tensor * q_w, const mi_tensor * q_out, const mi_tensor * k,
                              const mi_tensor * k_w, const mi_tensor * v, const mi_tensor * pos, float eps, int n_dims,
