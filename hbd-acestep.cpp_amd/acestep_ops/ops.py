@@ -269,8 +269,9 @@ def flash_attn_workspace(q, k, v) -> int:
 def flash_attn_ext(q, k, v, mask, scale: float, out=None, workspace=None, max_bias: float = 0.0,
                    logit_softcap: float = 0.0, stream=None):
     """ggml_flash_attn_ext (GGML_PREC_F32). Shapes outermost first:
-    q (N, Nh, n_q, D); k, v (Nk3, Nkv, n_kv, D) [or Q8]; mask F16 (mne3, mne2, >= n_q, n_kv) or None;
-    returns F32 (N, n_q, Nh, D) -- ggml's [D, Nh, n_q, N]. A workspace of the required size is
+    q (N, Nh, n_q, D); k, v (Nk3, Nkv, n_kv, D) [or Q8, Q4]; mask F16 (mne3, mne2, >= n_q, n_kv) or None;
+    returns F32 (N, n_q, Nh, D) -- ggml's [D, Nh, n_q, N] -- or fills `out`, which may be bf16 for
+    Q4 caches and bf16 q. A workspace of the required size is
     allocated when none is passed."""
     N, Nh, n_q, D = q.shape
     y = _out(out, (N, n_q, Nh, D), "f32")

@@ -784,7 +784,7 @@ static int fa_desc(const mi_tensor * q, const mi_tensor * k, const mi_tensor * v
         return MI_ERR_TYPE;
     }
     const int kt = k->type;
-    if (kt != v->type || (kt != MI_TYPE_F16 && kt != MI_TYPE_BF16 && kt != MI_TYPE_Q8_0 && kt != MI_TYPE_F32)) {
+    if (kt != v->type || (kt != MI_TYPE_F16 && kt != MI_TYPE_BF16 && !is_block(kt) && kt != MI_TYPE_F32)) {
         return MI_ERR_TYPE;
     }
     const int64_t D = q->ne[0];
@@ -801,8 +801,8 @@ static int fa_desc(const mi_tensor * q, const mi_tensor * k, const mi_tensor * v
         return MI_ERR_UNSUPPORTED;
     }
     // K/V rows are read in 16-byte chunks (Q8_0, 34-byte blocks: 8-byte when D is a
-    // multiple of 128, else 4-byte)
-    const size_t cb = kt == MI_TYPE_Q8_0 ? (D % 128 == 0 ? 8 : 4) : 16;
+    // multiple of 128, else 4-byte; Q4_0: 4-byte)
+    const size_t cb = kt == MI_TYPE_Q8_0 ? (D % 128 == 0 ? 8 : 4) : kt == MI_TYPE_Q4_0 ? 4 : 16;
     for (const mi_tensor * t : { k, v }) {
         if (!aligned(t->data, cb) || t->nb[1] % cb != 0 || t->nb[2] % cb != 0 || t->nb[3] % cb != 0) {
             return MI_ERR_ALIGN;
@@ -856,9 +856,10 @@ static int fa_desc(const mi_tensor * q, const mi_tensor * k, const mi_tensor * v
     }
     if (y) {
         MI_TRY(check(y));
-        if (y->type != MI_TYPE_F32) {
+        if (y->type != MI_TYPE_F32 && !(kt == MI_TYPE_Q4_0 && y->type == MI_TYPE_BF16 && q->type == MI_TYPE_BF16)) {
             return MI_ERR_TYPE;
         }
+        a.ty = y->type;
         if (y->ne[0] != D || y->ne[1] != q->ne[2] || y->ne[2] != q->ne[1] || y->ne[3] != q->ne[3]) {
             return MI_ERR_SHAPE;
         }

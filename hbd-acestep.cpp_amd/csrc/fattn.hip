@@ -2247,6 +2247,10 @@ static int fa_rb(int rows, int D, int kt) {
 // rows per wave and KV splits for a problem; the workspace holds one
 // (max, sum, D outputs) record per split and row when there is more than one split
 void flash_attn_plan(FaArgs & a, int D) {
+    if (a.kt == MI_TYPE_Q4_0) {
+        flash_attn_q4_plan(a, D);
+        return;
+    }
     a.rows          = a.n_q * a.rk;
     const int rb    = fa_rb(a.rows, D, a.kt);
     a.rblocks       = (a.rows + rb - 1) / rb;
@@ -2315,6 +2319,9 @@ size_t flash_attn_part_offset(const FaArgs & a) {
 }
 
 size_t flash_attn_workspace(const FaArgs & a, int D) {
+    if (a.kt == MI_TYPE_Q4_0) {
+        return flash_attn_q4_workspace(a, D);
+    }
     if (a.mfma) {  // the mask summary, sized for the largest mask a call may pass (one per batch and head),
                    // then the partials of split items
         return flash_attn_part_offset(a) + (size_t) a.tsplit * 2 * 128 * FA_PART * sizeof(float);
@@ -2378,6 +2385,9 @@ static int launch_k(const FaArgs & a, int D, hipStream_t s) {
 }
 
 int launch_flash_attn(const FaArgs & a, int kt, int D, hipStream_t s) {
+    if (kt == MI_TYPE_Q4_0) {
+        return launch_flash_attn_q4(a, D, s);
+    }
     if (a.rows == 0 || a.nb == 0 || a.nkv == 0) {
         return MI_OK;
     }

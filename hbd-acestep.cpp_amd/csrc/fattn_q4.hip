@@ -1,0 +1,650 @@
+// fattn_q4.hip -- flash attention over Q4_0 K and V (mi_flash_attn_ext).
+//
+//   s_ij = scale q_i . k_j + mask_ij,  y_i = sum_j softmax(s_i)_j v_j
+//
+// with k, v = (level - 8) d per block of 32 elements. Unlike a Q8_0 cache's, the
+// products take q as it is: a level has 4 bits, exact in fp16, so the matrix cores
+// multiply levels by q in fp16 and the block's d is applied to the fp32 sum.
+//  q      each row is scaled by a power of two so that its largest element is near
+//         2^13, then held as one fp16 (BF16 and F16 q, exact but for elements 2^-24
+//         of the row's largest) or as a high and a low one (F32 q, 22 bits).
+//  levels as fp16 operands are the nibbles themselves: 0x000n is n 2^-24 and 0x00n0
+//         16 n 2^-24, subnormals that the matrix cores take as they are, so two
+//         ANDs and a shift per pair make an operand; q's elements that meet a high
+//         nibble are divided by 16, 2^24 goes into the row's scale, and the -8 into
+//         the accumulator's start, -8 sum(q) of the block.
+//  P, V   F32 y: P and v = (level - 8) d as a high and a low fp16 each (v exact, P to
+//         22 bits), three products; BF16 y: one fp16 each (2^-11 against y's 2^-8).
+//         d above 8188 would leave fp16: tiles with one scale v by 2^-4, P by 2^4.
+// Sums, maxima and the running output are fp32.
+#include "launch.h"
+
+namespace mi {
+
+typedef _Float16 fa4_h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 fa4_h8 __attribute__((ext_vector_type(8)));
+typedef float    fa4_f4 __attribute__((ext_vector_type(4)));
+typedef int      fa4_v2i __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) fa4_v2i fa4_lds_v2i;
+typedef uint32_t fa4_u4 __attribute__((ext_vector_type(4), aligned(4)));  // rows are 4-byte aligned
+
+constexpr float FA4_LOG2E = 1.44269504088896340736f;
+constexpr float FA4_OFF   = 8.0f;   // p = exp2(s - max + 8): fp16 parts of p keep absolute 2^-32 of the largest
+constexpr float FA4_BIG   = 8188.0f;
+
+// the 18 bytes of block b (d, 16 bytes of levels) as loaded: 5 words from the 4-byte
+// boundary at or before the block, 20 bytes that never leave the row
+struct Fa4Raw {
+    uint32_t w[5];
+};
+
+__device__ __forceinline__ Fa4Raw fa4_load(const char * row, int blk) {
+    const char * p = row + ((18 * blk) & ~3);
+    const fa4_u4 x = *(const fa4_u4 *) p;
+    Fa4Raw       r;
+    r.w[0] = x.x;
+    r.w[1] = x.y;
+    r.w[2] = x.z;
+    r.w[3] = x.w;
+    r.w[4] = *(const uint32_t *) (p + 16);
+    return r;
+}
+
+// odd blocks start 2 bytes after the boundary: (d, levels) sit at bytes 2 and 4, even ones at 0 and 2
+__device__ __forceinline__ void fa4_block(const Fa4Raw & r, int blk, float & d, uint32_t * q) {
+    const uint32_t sel = blk & 1 ? 0x07060504u : 0x05040302u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        q[i] = __builtin_amdgcn_perm(r.w[i + 1], r.w[i], sel);
+    }
+    d = f16_lo(blk & 1 ? r.w[0] >> 16 : r.w[0]);
+}
+
+__device__ __forceinline__ uint32_t fa4_bits(fa4_h2 v) {
+    return __builtin_bit_cast(uint32_t, v);
+}
+
+__device__ __forceinline__ fa4_h2 fa4_half2(uint32_t v) {
+    return __builtin_bit_cast(fa4_h2, v);
+}
+
+// the B operand slots of one block of q: group g of the 4 lane groups takes bytes 4 g
+// .. 4 g + 3 of the levels; v: elements 4 g + (0..3), then 16 + 4 g + (0..3)
+__device__ __forceinline__ void fa4_slots(const float * v, float * s) {
+    s[0] = v[0];
+    s[1] = v[2];
+    s[2] = v[4] * 0.0625f;
+    s[3] = v[6] * 0.0625f;
+    s[4] = v[1];
+    s[5] = v[3];
+    s[6] = v[5] * 0.0625f;
+    s[7] = v[7] * 0.0625f;
+}
+
+// 8 levels of a word of 4 bytes as an A operand, in the slots' order
+__device__ __forceinline__ fa4_h8 fa4_levels(uint32_t w) {
+    const uint32_t v = w >> 8;
+    const u32x4    r = { w & 0x000f000fu, w & 0x00f000f0u, v & 0x000f000fu, v & 0x00f000f0u };
+    return __builtin_bit_cast(fa4_h8, r);
+}
+
+// the levels of keys (0, 2) and (1, 3) of a word (a byte per key) as fp16 numbers -8 .. 7:
+// the low nibbles, or the high ones. 0x6400 | n is 1024 + n.
+__device__ __forceinline__ fa4_h2 fa4_low(uint32_t w) {
+    const fa4_h2 c = { (_Float16) -1032.0f, (_Float16) -1032.0f };
+    return fa4_half2((w & 0x000f000fu) | 0x64006400u) + c;
+}
+
+__device__ __forceinline__ fa4_h2 fa4_high(uint32_t w) {
+    const fa4_h2 m = { (_Float16) 0.0625f, (_Float16) 0.0625f }, c = { (_Float16) -72.0f, (_Float16) -72.0f };
+    return __builtin_elementwise_fma(fa4_half2((w & 0x00f000f0u) | 0x64006400u), m, c);
+}
+
+// Query rows (query position, head) of a KV head in tiles of 16, keys split over
+// workgroups of W waves, a wave taking every (splits * W)-th tile of TK keys. With
+// v_mfma_f32_16x16x32_f16 (lane l: A[l%16][8(l/16)+e], B[8(l/16)+e][l%16],
+// C[4(l/16)+r][l%16]):
+//   S^T = K Q^T   A = levels of 16 keys from LDS, B = the 16 rows; one product per block
+//                 of 32 elements, each scaled by the keys' d. Lane l then holds the scores
+//                 of row l%16 for keys 16 mt + 4 (l/16) + r.
+//   O^T = V^T P^T B = those probabilities as they sit; A = the levels of V by transposed
+//                 8-bit LDS reads (lane l: byte l%16 of 8 keys, low nibble dim j, high
+//                 dim j + 16), times the keys' d.
+// The raw blocks of the next tile are in flight under the current one's math. Tiles with
+// no live key are not read where the 16 rows share a mask row (one query position), and
+// a key that no row attends to counts as v = 0 whatever its bytes are.
+template <int D> struct Fa4 {
+    static constexpr int NB   = D / 32;
+    static constexpr int TK   = D == 256 ? 32 : 64;  // keys per tile
+    static constexpr int IPL  = TK * NB / 64;        // blocks per lane and tile, of K and of V
+    static constexpr int MT   = TK / 16;
+    static constexpr int KROW = 16 * NB;             // bytes of levels per key
+    static constexpr int RPP  = 16 / NB;             // keys per padding
+    static constexpr int DS   = TK + 64 / NB;        // entries per block in the tables of d
+    static constexpr int KB   = TK * KROW + TK / RPP * 4 * NB;
+    static constexpr int VB   = TK * KROW + TK / RPP * 16;
+    static constexpr int DKB  = NB * DS * 4;
+    static constexpr int DVB  = NB * DS * 2;
+    static constexpr int MB   = 8;                   // tiles whose mask is read at once
+    static constexpr int WAVE = KB + VB + DKB + DVB; // LDS bytes per wave, without the mask
+    static constexpr int DC   = D < 128 ? D : 128;   // columns merged at a time
+    static __device__ __forceinline__ int koff(int key) { return key * KROW + key / RPP * 4 * NB; }
+    static __device__ __forceinline__ int voff(int key) { return key * KROW + key / RPP * 16; }
+};
+
+// MS: 0 no mask, 1 one mask row for all rows of the tile, 2 a mask row each
+template <int D, int QP, bool OS, int MS, int W>
+__global__ void __launch_bounds__(64 * W) k_fa4_dec(const FaArgs a) {
+    using F           = Fa4<D>;
+    constexpr int NB  = F::NB, TK = F::TK, IPL = F::IPL, MT = F::MT;
+    constexpr int MSB = MS == 1 ? F::MB * TK * 4 : 0;
+    constexpr int WB  = F::WAVE + MSB;
+    static_assert(WB >= 16 * F::DC * 4, "the merge reuses the tiles' memory");
+    __shared__ __align__(16) char lds[W * WB];
+    __shared__ float              stat[W][16][2];
+
+    const int      lane = threadIdx.x & 63;
+    const int      wv   = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int      c16 = lane & 15, q4 = lane >> 4;
+    const uint32_t item  = blockIdx.x / (uint32_t) a.splits;
+    const uint32_t split = blockIdx.x - item * (uint32_t) a.splits;
+    const uint32_t bg    = item / (uint32_t) a.rblocks;
+    const int      rt    = (int) (item - bg * (uint32_t) a.rblocks);
+    const uint32_t b     = bg / (uint32_t) a.nkv;
+    const uint32_t g     = bg - b * (uint32_t) a.nkv;
+    const int      row   = rt * 16 + c16 < a.rows ? rt * 16 + c16 : a.rows - 1;  // past the end: the last row again
+    const int      iq    = row / a.rk;
+    const int      h     = (int) g * a.rk + (row - iq * a.rk);
+    const uint32_t kb    = b / (uint32_t) a.rk3;
+    const char *   kg    = a.k + (int64_t) kb * a.k3 + (int64_t) g * a.k2;
+    const char *   vg    = a.v + (int64_t) kb * a.v3 + (int64_t) g * a.v2;
+    const char *   mrow  = nullptr;
+    if constexpr (MS != 0) {
+        mrow = a.mask + (int64_t) (b % (uint32_t) a.mne3) * a.m3 + (int64_t) (h % a.mne2) * a.m2 + (int64_t) iq * a.m1;
+    }
+    char *  kl  = lds + wv * WB;
+    char *  vl  = kl + F::KB;
+    float * dkl = (float *) (vl + F::VB);
+    char *  dvl = (char *) dkl + F::DKB;
+    float * ml  = (float *) (dvl + F::DVB);
+
+    // q: this lane's 8 elements of each block, the row's largest magnitude over the 4 lane groups
+    float qv[NB][8];
+    {
+        const char * qp = a.q + (int64_t) b * a.q3 + (int64_t) h * a.q2 + (int64_t) iq * a.q1;
+#pragma unroll
+        for (int blk = 0; blk < NB; ++blk) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int i = blk * 32 + 4 * q4 + (e & 3) + (e & 4) * 4;
+                qv[blk][e]  = a.tq == MI_TYPE_F32    ? load_elem<MI_TYPE_F32>(qp + (size_t) i * 4)
+                              : a.tq == MI_TYPE_BF16 ? load_elem<MI_TYPE_BF16>(qp + (size_t) i * 2)
+                                                     : load_elem<MI_TYPE_F16>(qp + (size_t) i * 2);
+            }
+        }
+    }
+    float qmax = 0.0f;
+#pragma unroll
+    for (int blk = 0; blk < NB; ++blk) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            qmax = fmaxf(qmax, fabsf(qv[blk][e]));
+        }
+    }
+    qmax     = fmaxf(qmax, __shfl_xor(qmax, 16, 64));
+    qmax     = fmaxf(qmax, __shfl_xor(qmax, 32, 64));
+    int ex   = (int) (__float_as_uint(qmax) >> 23) - 127;  // 2^ex <= qmax < 2^(ex + 1)
+    ex       = ex < -100 ? -100 : ex > 127 ? 13 : ex;      // a row that is not finite: as it is
+    const float up = __uint_as_float((uint32_t) (127 + 13 - ex) << 23);
+    const float qs = a.scale * FA4_LOG2E * __uint_as_float((uint32_t) (127 - 13 + ex) << 23);
+    fa4_h8      qb[QP][NB];
+    float       c0[NB];
+#pragma unroll
+    for (int blk = 0; blk < NB; ++blk) {
+        float s[8], sum = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            qv[blk][e] *= up;
+        }
+        fa4_slots(qv[blk], s);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const _Float16 hi = (_Float16) s[e];
+            qb[0][blk][e]     = hi;
+            float used        = (float) hi;
+            if constexpr (QP == 2) {
+                const _Float16 lo = (_Float16) (s[e] - (float) hi);
+                qb[1][blk][e]     = lo;
+                used += (float) lo;
+            }
+            sum += e & 2 ? used * 16.0f : used;  // slots 2, 3, 6, 7 meet 16 times the level
+        }
+        sum += __shfl_xor(sum, 16, 64);
+        sum += __shfl_xor(sum, 32, 64);
+        c0[blk] = sum * (-8.0f / 16777216.0f);
+    }
+
+    float  m = -INFINITY, l = 0.0f;
+    fa4_f4 o[2 * NB];
+#pragma unroll
+    for (int i = 0; i < 2 * NB; ++i) {
+        o[i] = fa4_f4{ 0.0f, 0.0f, 0.0f, 0.0f };
+    }
+
+    const int ntile = (a.n_kv + TK - 1) / TK;
+    const int step  = a.splits * W;
+    Fa4Raw    kr[IPL], vr[IPL];
+    uint16_t  mr[MS == 2 ? MT : 1][4];
+    auto      load = [&](int t) {
+        const int t0 = t * TK, last = a.n_kv - 1 - t0;
+#pragma unroll
+        for (int i = 0; i < IPL; ++i) {
+            const int     idx = i * 64 + lane, blk = idx % NB;
+            const int     key = idx / NB < last ? idx / NB : last;  // past the end: the last key again
+            const int64_t at  = (int64_t) (t0 + key);
+            kr[i]             = fa4_load(kg + at * a.k1, blk);
+            vr[i]             = fa4_load(vg + at * a.v1, blk);
+        }
+        if constexpr (MS == 2) {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int key = 16 * mt + 4 * q4 + r;
+                    mr[mt][r]     = *(const uint16_t *) (mrow + (int64_t) (t0 + (key < last ? key : last)) * 2);
+                }
+            }
+        }
+    };
+
+    for (int base = (int) split * W + wv; base < ntile; base += F::MB * step) {
+        uint32_t todo = 0;  // bit i: tile base + i * step is to be walked
+        if constexpr (MS == 1) {
+            uint16_t mv[F::MB];
+#pragma unroll
+            for (int i = 0; i < F::MB; ++i) {
+                const int key = (base + i * step) * TK + (lane & (TK - 1));
+                mv[i]         = *(const uint16_t *) (mrow + (int64_t) (key < a.n_kv ? key : a.n_kv - 1) * 2);
+            }
+#pragma unroll
+            for (int i = 0; i < F::MB; ++i) {
+                const int   key = (base + i * step) * TK + (lane & (TK - 1));
+                const float x   = key < a.n_kv ? f16_lo(mv[i]) * FA4_LOG2E : -INFINITY;
+                todo |= (uint32_t) (__builtin_amdgcn_ballot_w64(x != -INFINITY) != 0) << i;
+                if (lane < TK) {
+                    ml[i * TK + lane] = x;
+                }
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+        } else {
+            const int n = (ntile - base + step - 1) / step;
+            todo        = n >= F::MB ? (1u << F::MB) - 1 : (1u << n) - 1;
+        }
+        if (todo) {
+            load(base + (__builtin_ffs(todo) - 1) * step);
+        }
+        while (todo) {
+            const int i = __builtin_ffs(todo) - 1;
+            todo &= todo - 1;
+            const int t0 = (base + i * step) * TK;
+            // mask values of this lane's scores, and the keys that some row attends to
+            float    ms[MT][4];
+            uint64_t live = 0;
+            if constexpr (MS == 1) {
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    const fa4_f4 x = *(const fa4_f4 *) (ml + i * TK + 16 * mt + 4 * q4);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        ms[mt][r] = x[r];
+                    }
+                }
+                live = __builtin_amdgcn_ballot_w64(ml[i * TK + (lane & (TK - 1))] != -INFINITY);
+            } else {
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const bool in = t0 + 16 * mt + 4 * q4 + r < a.n_kv;
+                        ms[mt][r]     = !in ? -INFINITY : MS == 2 ? f16_lo(mr[MS == 2 ? mt : 0][r]) * FA4_LOG2E : 0.0f;
+                        const uint64_t v = __builtin_amdgcn_ballot_w64(ms[mt][r] != -INFINITY);
+#pragma unroll
+                        for (int gr = 0; gr < 4; ++gr) {
+                            live |= (uint64_t) ((v >> (16 * gr) & 0xffffu) != 0) << (16 * mt + 4 * gr + r);
+                        }
+                    }
+                }
+            }
+            // raw blocks to LDS: K's levels as words [key][group][block], V's as rows, d by block and key
+            bool big = false;
+#pragma unroll
+            for (int it = 0; it < IPL; ++it) {
+                const int idx = it * 64 + lane, key = idx / NB, blk = idx % NB;
+                float     d;
+                uint32_t  q[4];
+                fa4_block(kr[it], blk, d, q);
+                char * kp = kl + F::koff(key) + blk * 4;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    *(uint32_t *) (kp + e * 4 * NB) = q[e];
+                }
+                dkl[blk * F::DS + key] = d * 16777216.0f;
+                fa4_block(vr[it], blk, d, q);
+                *(uint4 *) (vl + F::voff(key) + blk * 16) = make_uint4(q[0], q[1], q[2], q[3]);
+                d   = live >> key & 1 ? d : 0.0f;
+                big = big || fabsf(d) > FA4_BIG;
+                // in the order of the slots: keys 0, 2, 1, 3 of each four
+                const int kp4 = (key & ~3) | (key & 1) << 1 | (key >> 1 & 1);
+                *(_Float16 *) (dvl + (blk * F::DS + kp4) * 2) = (_Float16) d;
+            }
+            big = __builtin_amdgcn_ballot_w64(big) != 0;
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            if (todo) {
+                load(base + (__builtin_ffs(todo) - 1) * step);
+            }
+
+            // scores, in units of log2
+            float s[MT][4], mx = -INFINITY;
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                const uint32_t * kp = (const uint32_t *) (kl + F::koff(16 * mt + c16) + q4 * 4 * NB);
+                uint32_t         kw[NB];
+#pragma unroll
+                for (int blk = 0; blk < NB; ++blk) {
+                    kw[blk] = kp[blk];
+                }
+                fa4_f4 t = { 0.0f, 0.0f, 0.0f, 0.0f };
+#pragma unroll
+                for (int blk = 0; blk < NB; ++blk) {
+                    const fa4_h8 x   = fa4_levels(kw[blk]);
+                    fa4_f4       acc = { c0[blk], c0[blk], c0[blk], c0[blk] };
+#pragma unroll
+                    for (int p = 0; p < QP; ++p) {
+                        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, qb[p][blk], acc, 0, 0, 0);
+                    }
+                    const fa4_f4 dk = *(const fa4_f4 *) (dkl + blk * F::DS + 16 * mt + 4 * q4);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        t[r] = __builtin_fmaf(acc[r], dk[r], t[r]);
+                    }
+                }
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    s[mt][r] = ms[mt][r] == -INFINITY ? -INFINITY : __builtin_fmaf(t[r], qs, ms[mt][r]);
+                    mx       = fmaxf(mx, s[mt][r]);
+                }
+            }
+            mx                = fmaxf(mx, __shfl_xor(mx, 16, 64));
+            mx                = fmaxf(mx, __shfl_xor(mx, 32, 64));
+            const float mnew  = fmaxf(m, mx);
+            const float mu    = (mnew == -INFINITY ? 0.0f : mnew) - FA4_OFF;
+            if (__builtin_amdgcn_ballot_w64(mnew > m) != 0) {
+                const float al = m == mnew ? 1.0f : __builtin_amdgcn_exp2f(m - mnew);
+                l *= al;
+#pragma unroll
+                for (int j = 0; j < 2 * NB; ++j) {
+                    o[j] *= al;
+                }
+                m = mnew;
+            }
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    s[mt][r] = __builtin_amdgcn_exp2f(s[mt][r] - mu);
+                    l += s[mt][r];
+                }
+            }
+            if (big) {  // d / 16 held in fp16, p * 16
+#pragma unroll
+                for (int it = 0; it < IPL; ++it) {
+                    const int idx = it * 64 + lane, key = idx / NB, blk = idx % NB;
+                    const int kp4 = (key & ~3) | (key & 1) << 1 | (key >> 1 & 1);
+                    _Float16 * dp = (_Float16 *) (dvl + (blk * F::DS + kp4) * 2);
+                    *dp           = *dp * (_Float16) 0.0625f;
+                }
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        s[mt][r] *= 16.0f;
+                    }
+                }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+            }
+#pragma unroll
+            for (int kgp = 0; kgp < TK / 32; ++kgp) {
+                fa4_h8 ph, pl;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {  // slots: keys 0, 2, 1, 3 of each four
+                    const float p = s[2 * kgp + e / 4][(e & 1) * 2 + (e >> 1 & 1)];
+                    ph[e]         = (_Float16) p;
+                    if constexpr (OS) {
+                        pl[e] = (_Float16) (p - (float) ph[e]);
+                    }
+                }
+                // lane m of a group of 16 addresses key m / 2 of the group's 8, half m % 2 of a block's 16 bytes
+                const int mk  = c16 >> 1;
+                const int key = 32 * kgp + 4 * q4 + (mk & 3) + (mk & 4) * 4;
+                char *    vp  = vl + F::voff(key) + 8 * (c16 & 1);
+#pragma unroll
+                for (int blk = 0; blk < NB; ++blk) {
+                    const fa4_v2i  w  = __builtin_amdgcn_ds_read_tr8_b64_v2i32((fa4_lds_v2i *) (vp + blk * 16));
+                    const uint32_t w0 = (uint32_t) w.x, w1 = (uint32_t) w.y;
+                    const uint2    da = *(const uint2 *) (dvl + (blk * F::DS + 32 * kgp + 4 * q4) * 2);
+                    const uint2    db = *(const uint2 *) (dvl + (blk * F::DS + 32 * kgp + 16 + 4 * q4) * 2);
+                    const uint32_t dd[4] = { da.x, da.y, db.x, db.y };
+                    const uint32_t ww[4] = { w0, w0 >> 8, w1, w1 >> 8 };
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        u32x4 vh, vlo;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const fa4_h2 x = half ? fa4_high(ww[e]) : fa4_low(ww[e]);
+                            const fa4_h2 d = fa4_half2(dd[e]), v = x * d;
+                            vh[e] = fa4_bits(v);
+                            if constexpr (OS) {
+                                vlo[e] = fa4_bits(__builtin_elementwise_fma(x, d, -v));
+                            }
+                        }
+                        const fa4_h8 av = __builtin_bit_cast(fa4_h8, vh);
+                        fa4_f4 &     oo = o[2 * blk + half];
+                        oo              = __builtin_amdgcn_mfma_f32_16x16x32_f16(av, ph, oo, 0, 0, 0);
+                        if constexpr (OS) {
+                            oo = __builtin_amdgcn_mfma_f32_16x16x32_f16(av, pl, oo, 0, 0, 0);
+                            oo = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(fa4_h8, vlo), ph, oo, 0, 0, 0);
+                        }
+                    }
+                }
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+        }
+    }
+
+    // merge the waves: (m, l) of each row, then the outputs relative to the largest m
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    if (q4 == 0) {
+        stat[wv][c16][0] = m;
+        stat[wv][c16][1] = l;
+    }
+    __syncthreads();
+    float mm = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+        mm = fmaxf(mm, stat[w][c16][0]);
+    }
+    const float wt = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mm);
+    const int   nr = a.rows - rt * 16 < 16 ? a.rows - rt * 16 : 16;
+    constexpr int DC = F::DC;
+#pragma unroll
+    for (int c = 0; c < D / DC; ++c) {
+        if (c > 0) {
+            __syncthreads();
+        }
+        float * om = (float *) (lds + wv * WB);
+#pragma unroll
+        for (int j = 0; j < DC / 16; ++j) {
+            *(fa4_f4 *) (om + c16 * DC + j * 16 + 4 * q4) = o[c * (DC / 16) + j] * wt;
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < nr * DC; i += 64 * W) {
+            const int r = i / DC, d = i - r * DC;
+            float     acc = 0.0f, mr2 = -INFINITY, ls = 0.0f;
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                acc += ((const float *) (lds + w * WB))[i];
+                mr2 = fmaxf(mr2, stat[w][r][0]);
+            }
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                const float mw = stat[w][r][0];
+                ls += mw == -INFINITY ? 0.0f : stat[w][r][1] * __builtin_amdgcn_exp2f(mw - mr2);
+            }
+            const int rr = rt * 16 + r;
+            if (a.splits > 1) {
+                float * p = a.ws + (((int64_t) bg * a.rows + rr) * a.splits + split) * (D + 4);
+                if (c == 0 && d == 0) {
+                    p[0] = mr2;
+                    p[1] = ls;
+                }
+                p[4 + c * DC + d] = acc;
+            } else {
+                const int iq2 = rr / a.rk, h2 = (int) g * a.rk + (rr - iq2 * a.rk);
+                char *    yp  = a.y + (int64_t) b * a.y3 + (int64_t) iq2 * a.y2 + (int64_t) h2 * a.y1;
+                const float v = acc / ls;  // no live key: 0 / 0
+                if (a.ty == MI_TYPE_F32) {
+                    store_elem<MI_TYPE_F32>(yp + (size_t) (c * DC + d) * 4, v);
+                } else {
+                    store_elem<MI_TYPE_BF16>(yp + (size_t) (c * DC + d) * 2, v);
+                }
+            }
+        }
+    }
+}
+
+// The splits' partial results of a row: y = sum_i w_i o_i / sum_i w_i l_i with w_i =
+// exp2(m_i - max m). A wave per row, a lane per D / 64 columns.
+template <int D>
+__global__ void __launch_bounds__(64) k_fa4_combine(const FaArgs a) {
+    constexpr int  C    = D / 64;
+    const int      lane = threadIdx.x;
+    const uint32_t rec  = blockIdx.x;
+    const uint32_t bg   = rec / (uint32_t) a.rows;
+    const int      row  = (int) (rec - bg * (uint32_t) a.rows);
+    const uint32_t b    = bg / (uint32_t) a.nkv;
+    const uint32_t g    = bg - b * (uint32_t) a.nkv;
+    const int      iq   = row / a.rk;
+    const int      h    = (int) g * a.rk + (row - iq * a.rk);
+    const float *  p    = a.ws + (int64_t) rec * a.splits * (D + 4);
+    float          m = -INFINITY, l = 0.0f, acc[C] = {};
+    for (int s0 = 0; s0 < a.splits; s0 += 64) {
+        const int   n  = a.splits - s0 < 64 ? a.splits - s0 : 64;
+        const int   s  = s0 + (lane < n ? lane : n - 1);
+        const float ms = lane < n ? p[(int64_t) s * (D + 4)] : -INFINITY;
+        const float ls = p[(int64_t) s * (D + 4) + 1];
+        const float mn = fmaxf(m, group_max<64>(ms));
+        const float al = m == mn ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+        const float w  = ms == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ms - mn);
+        l              = __builtin_fmaf(l, al, group_sum<64>(w == 0.0f ? 0.0f : w * ls));
+        m              = mn;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            acc[c] *= al;
+        }
+        for (int j = 0; j < n; ++j) {
+            const float   wj = __shfl(w, j, 64);
+            const float * op = p + (int64_t) (s0 + j) * (D + 4) + 4 + lane * C;
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                acc[c] = __builtin_fmaf(wj, op[c], acc[c]);
+            }
+        }
+    }
+    char * yp = a.y + (int64_t) b * a.y3 + (int64_t) iq * a.y2 + (int64_t) h * a.y1;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const float v = acc[c] / l;  // no live key: 0 / 0
+        if (a.ty == MI_TYPE_F32) {
+            store_elem<MI_TYPE_F32>(yp + (size_t) (lane * C + c) * 4, v);
+        } else {
+            store_elem<MI_TYPE_BF16>(yp + (size_t) (lane * C + c) * 2, v);
+        }
+    }
+}
+
+constexpr int FA4_W = 4;  // waves per workgroup
+
+void flash_attn_q4_plan(FaArgs & a, int D) {
+    a.rows    = a.n_q * a.rk;
+    a.rblocks = (a.rows + 15) / 16;
+    a.splits  = 1;
+    const int     tk     = D == 256 ? 32 : 64;
+    const int64_t items  = (int64_t) a.nb * a.nkv * a.rblocks;
+    const int64_t tiles  = ((int64_t) a.n_kv + tk - 1) / tk;
+    if (items == 0 || tiles == 0) {
+        return;
+    }
+    if (a.n_kv > 1 << 27) {
+        a.splits = 0;  // a wave's walk counts keys in 32 bits, 8 tiles of every wave ahead
+        return;
+    }
+    // enough waves for 16 per CU, at most one tile each
+    const int64_t want = ((int64_t) num_cus() * 16 / FA4_W + items - 1) / items;
+    const int64_t most = (tiles + FA4_W - 1) / FA4_W;
+    a.splits           = (int) (want < most ? want : most);
+    if (items * a.splits >= ((int64_t) 1 << 31)) {
+        a.splits = 0;  // more workgroups than a grid has
+    }
+}
+
+size_t flash_attn_q4_workspace(const FaArgs & a, int D) {
+    return a.splits > 1 ? (size_t) a.splits * a.nb * a.nkv * a.rows * (D + 4) * sizeof(float) : 0;
+}
+
+template <int D, int QP, bool OS>
+static void launch_dec(const FaArgs & a, hipStream_t s) {
+    const dim3 grid((uint32_t) ((int64_t) a.nb * a.nkv * a.rblocks * a.splits)), wg(64 * FA4_W);
+    if (a.mask == nullptr) {
+        MI_LAUNCH((k_fa4_dec<D, QP, OS, 0, FA4_W>), grid, wg, 0, s, a);
+    } else if (a.n_q == 1 && a.mne2 == 1) {
+        MI_LAUNCH((k_fa4_dec<D, QP, OS, 1, FA4_W>), grid, wg, 0, s, a);
+    } else {
+        MI_LAUNCH((k_fa4_dec<D, QP, OS, 2, FA4_W>), grid, wg, 0, s, a);
+    }
+    if (a.splits > 1) {
+        MI_LAUNCH((k_fa4_combine<D>), dim3((uint32_t) (a.nb * a.nkv * a.rows)), dim3(64), 0, s, a);
+    }
+}
+
+template <int D>
+static int launch_d(const FaArgs & a, hipStream_t s) {
+    if (a.ty == MI_TYPE_BF16) {
+        launch_dec<D, 1, false>(a, s);
+    } else if (a.tq == MI_TYPE_F32) {
+        launch_dec<D, 2, true>(a, s);
+    } else {
+        launch_dec<D, 1, true>(a, s);
+    }
+    return MI_OK;
+}
+
+int launch_flash_attn_q4(const FaArgs & a, int D, hipStream_t s) {
+    if (a.rows == 0 || a.nb == 0 || a.nkv == 0) {
+        return MI_OK;
+    }
+    switch (D) {
+        case 64:
+            return launch_d<64>(a, s);
+        case 128:
+            return launch_d<128>(a, s);
+        default:
+            return launch_d<256>(a, s);
+    }
+}
+
+}  // namespace mi

@@ -158,7 +158,8 @@ struct FaArgs {
     int          ngq;      // matrix-core path: groups of 16 query positions in the mask summary
     uint8_t *    msum;     // matrix-core path with a mask: per (mask batch, mask head, group, key tile)
                            // bit 0 = some key not -inf, bit 1 = some value not 0 (in the workspace)
-    char *       y;  // F32 [D, Nh, n_q, N]: y1 = head, y2 = position, y3 = batch
+    char *       y;  // [D, Nh, n_q, N]: y1 = head, y2 = position, y3 = batch
+    int          ty; // F32, or BF16 (Q4_0 K/V and BF16 q)
     int64_t      y1, y2, y3;
     int          n_q, n_kv, nh, nkv, nb, rk, rk3;
     int          kt;  // K and V type
@@ -176,6 +177,10 @@ void   flash_attn_plan(FaArgs & a, int D);
 size_t flash_attn_workspace(const FaArgs & a, int D);
 size_t flash_attn_part_offset(const FaArgs & a);
 int    launch_flash_attn(const FaArgs & a, int kt, int D, hipStream_t s);
+// Q4_0 K and V (fattn_q4.hip); the three above call these
+void   flash_attn_q4_plan(FaArgs & a, int D);
+size_t flash_attn_q4_workspace(const FaArgs & a, int D);
+int    launch_flash_attn_q4(const FaArgs & a, int D, hipStream_t s);
 
 // ---- matmul.hip ------------------------------------------------------------
 // ggml_mul_mat(w, x), Q8_0 weights in the R64 layout, F32 x rows

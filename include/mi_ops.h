@@ -243,17 +243,19 @@ int mi_timestep_embedding(const mi_tensor * t, int dim, int max_period, const mi
  * batched decode attention over it (qwen3-lm.h:718-723, 256-bucketed read
  * length at 582-596; songgen-lelm-gen.h:582-583).
  *   q:    [D, n_q, Nh, N]      F32/BF16/F16
- *   k, v: [D, n_kv, Nkv, Nk3]  both F16, both BF16, both Q8_0 or both F32
- *         (F32 only for D <= 128); Nh % Nkv == 0, N % Nk3 == 0; rows at a
+ *   k, v: [D, n_kv, Nkv, Nk3]  both F16, both BF16, both Q8_0, both Q4_0 or both
+ *         F32 (F32 only for D <= 128); Nh % Nkv == 0, N % Nk3 == 0; rows at a
  *         16-byte aligned stride (Q8_0: 8-byte when D % 128 == 0, else
- *         4-byte), e.g. cache views
+ *         4-byte; Q4_0: 4-byte), e.g. cache views
  *   mask: F16 [n_kv, >= n_q, mne2, mne3] (head h uses h % mne2, batch b uses
  *         b % mne3) or NULL
- *   y:    F32 [D, Nh, n_q, N]  (ggml's permuted result)
+ *   y:    F32 [D, Nh, n_q, N]  (ggml's permuted result); BF16 too with Q4_0 K
+ *         and V and BF16 q
  * D (= ne0 of q, k and v) is 64, 128 or 256. max_bias and logit_softcap must
  * be 0 (the only values the reference passes); others return
  * MI_ERR_UNSUPPORTED. q is converted to K's dot type as ggml-cpu converts it
- * (fp16, bf16, or Q8_0 with the x86 rounding); keys whose mask is -inf do not
+ * (fp16, bf16, or Q8_0 with the x86 rounding; with Q4_0 K it is used as it is,
+ * to 22 bits of an F32 row's largest element); keys whose mask is -inf do not
  * contribute; a row whose keys are all masked is NaN. The decode and split
  * kernels never read masked keys; the matrix-core prefill kernel (64 or more
  * (query, head) rows per KV head, D = 128) reads the K/V rows of keys masked

@@ -97,3 +97,32 @@ def test_descriptors_of_block_views(typ, bsz):
     assert list(d.nb) == [bsz, 4 * bsz, 64 * 4 * bsz, 3 * 64 * 4 * bsz] and w.shape == (2, 3, 40, 128)
     with pytest.raises(ValueError):
         ops.desc((ops.Q4 if typ == Q8_0 else ops.Q8)(x))
+
+
+def test_attention_refused():
+    D, n_q, nh, nkv, n, N = 128, 3, 8, 2, 100, 2
+    q, k, v, y = _t([D, n_q, nh, N], BF16), _t([D, n, nkv, N], Q4_0), _t([D, n, nkv, N], Q4_0), _t([D, nh, n_q, N])
+
+    def fa(q=q, k=k, v=v, y=y, mask=None, scale=0.1):
+        return L.mi_flash_attn_ext(R(q), R(k), R(v), R(mask) if mask else None, scale, 0.0, 0.0, R(y), None, 0, None)
+
+    assert fa(v=_t([D, n, nkv, N], Q8_0)) == -2                                      # K and V of two types
+    assert fa(y=_t([D, nh, n_q, N], F16)) == -2
+    assert fa(q=_t([D, n_q, nh, N]), y=_t([D, nh, n_q, N], BF16)) == -2              # BF16 y needs BF16 q
+    assert fa(k=_t([D, n, nkv, N], F16), v=_t([D, n, nkv, N], F16), y=_t([D, nh, n_q, N], BF16)) == -2
+    assert fa(k=_t([D, n, nkv, N], Q4_0, data=4098)) == -5                           # rows at a 4-byte boundary
+    assert fa(k=_t([D, n, nkv, N], Q4_0, nb=[18, 74, 7400, 14800])) == -5
+    assert fa(q=_t([96, n_q, nh, N]), k=_t([96, n, nkv, N], Q4_0), v=_t([96, n, nkv, N], Q4_0), y=_t([96, nh, n_q, N])) == -7
+    assert fa(k=_t([D, n, 3, N], Q4_0), v=_t([D, n, 3, N], Q4_0)) == -3
+    assert fa(scale=float("nan")) == -6
+    assert fa(mask=_t([n, n_q - 1, 1, 1], F16)) == -3
+    big = _t([D, 1 << 28, nkv, N], Q4_0)
+    assert fa(k=big, v=big) == -7
+    # long caches with few heads are split: a workspace is needed
+    one, long = _t([D, 1, nh, N]), _t([D, 20000, nkv, N], Q4_0)
+    nb = ctypes.c_size_t(0)
+    assert L.mi_flash_attn_ext_workspace(R(one), R(long), R(long), ctypes.byref(nb)) == 0 and nb.value > 0
+    yo = _t([D, nh, 1, N])
+    assert L.mi_flash_attn_ext(R(one), R(long), R(long), None, 0.1, 0.0, 0.0, R(yo), None, 0, None) == -6
+    assert L.mi_flash_attn_ext(R(one), R(long), R(long), None, 0.1, 0.0, 0.0, R(yo), ctypes.c_void_p(4097),
+                               nb.value, None) == -5
