@@ -130,6 +130,9 @@ PROTOTYPES = {
                                    _TP, _VP, ctypes.c_size_t, _VP],
     "mi_mul_mat_q8_0_swiglu_gated_add": [_VP, ctypes.c_int64, ctypes.c_int64, _TP, ctypes.c_int, _TP, _TP, _TP, _VP,
                                          ctypes.c_size_t, _VP],
+    "mi_lora_add_workspace": [_TP, _TP, _TP, ctypes.POINTER(ctypes.c_size_t)],
+    "mi_lora_add": [_TP, _TP, _TP, _TP, _TP, _TP, _TP, _VP, ctypes.c_size_t, _VP, _VP],
+    "mi_logits_adjust": [_TP, _TP, _TP, _TP, _TP, _TP, _TP, _TP, _VP, _VP],
     "mi_apg_buffer_bytes": [_TP, ctypes.POINTER(ctypes.c_size_t)],
     "mi_apg_forward": [_TP, _TP, _F, _F, _F, _VP, ctypes.c_size_t, _I, _TP, _VP],
     "mi_flow_step": [_I, _TP, _TP, _F, _F, _I, _TP, _TP, _VP],

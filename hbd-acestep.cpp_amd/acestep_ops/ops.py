@@ -435,3 +435,35 @@ def mul_mat_q8_0(w: Q8R64, x, out=None, workspace=None, stream=None):
     wn = ws.numel() * ws.es if ws is not None else 0
     _lib.call("mi_mul_mat_q8_0", ctypes.c_void_p(w.data.ptr), w.k, w.n, _p(x), _p(y), wp, wn, _s(stream))
     return y
+
+
+def lora_add_workspace(x, a, b) -> int:
+    """Bytes of device workspace mi_lora_add needs for these operands."""
+    nb = ctypes.c_size_t(0)
+    _lib.call("mi_lora_add_workspace", _p(x), _p(a), _p(b), ctypes.byref(nb))
+    return int(nb.value)
+
+
+def lora_add(y0, x, a, b, ids, scales=None, out=None, workspace=None, err=None, stream=None):
+    """y0 + scales[id] * B[id] (A[id] x) with each row's own adapter: x F32 (m, k), y0 F32 (m, n),
+    a (n_adapters, r, k) and b (n_adapters, n, r) bf16 or f16, ids i32 (m,), negative: none.
+    `out` may be y0. A workspace of the required size is allocated when none is passed."""
+    y = _out(out, y0.shape, "f32")
+    ws = workspace if workspace is not None else DTensor.empty((max(lora_add_workspace(x, a, b), 16),), "u8")
+    ep = ctypes.c_void_p(err.ptr) if err is not None else None
+    _lib.call("mi_lora_add", _p(y0), _p(x), _p(a), _p(b), _p(ids), _p(scales), _p(y), ctypes.c_void_p(ws.ptr),
+              ws.numel() * ws.es, ep, _s(stream))
+    return y
+
+
+def logits_adjust(logits, history=None, lengths=None, penalties=None, bias=None, allowed=None, state=None, out=None,
+                  err=None, stream=None):
+    """Penalties for tokens of the history, a bias and a grammar's mask on logits (rows, n_vocab):
+    history i32 (rows, n), lengths i32 (rows,), penalties F32 (rows, 3) = (repetition, frequency,
+    presence), bias F32 (n_vocab,), (1, n_vocab) or (rows, n_vocab), allowed i32 (n_states, words) with a
+    bit per token, state i32 (rows,), negative: no grammar. `out` may be logits."""
+    y = _out(out, logits.shape, logits.dtype)
+    ep = ctypes.c_void_p(err.ptr) if err is not None else None
+    _lib.call("mi_logits_adjust", _p(logits), _p(history), _p(lengths), _p(penalties), _p(bias), _p(allowed), _p(state),
+              _p(y), ep, _s(stream))
+    return y

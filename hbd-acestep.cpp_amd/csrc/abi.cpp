@@ -1331,6 +1331,226 @@ static int lat_check(const mi_tensor * x, const mi_tensor * ref) {
     return MI_OK;
 }
 
+static int check_i32(const mi_tensor * t, int64_t n, bool inner) {
+    MI_TRY(check(t, inner));
+    if (t->type != MI_TYPE_I32) {
+        return MI_ERR_TYPE;
+    }
+    return t->ne[0] == n && t->ne[1] == 1 && t->ne[2] == 1 && t->ne[3] == 1 ? MI_OK : MI_ERR_SHAPE;
+}
+
+// bytes [lo, hi) that a view addresses
+static void view_span(const mi_tensor & t, uintptr_t & lo, uintptr_t & hi) {
+    lo = hi = (uintptr_t) t.data;
+    if (nelements(t) == 0) {
+        return;
+    }
+    hi += (uintptr_t) type_size(t.type);
+    for (int d = 0; d < 4; ++d) {
+        hi += (uintptr_t) ((d == 0 ? t.ne[0] / blck_size(t.type) : t.ne[d]) - 1) * t.nb[d];
+    }
+}
+
+static bool views_overlap(const mi_tensor & a, const mi_tensor & b) {
+    uintptr_t a0, a1, b0, b1;
+    view_span(a, a0, a1);
+    view_span(b, b0, b1);
+    return a0 < b1 && b0 < a1;
+}
+
+static bool same_view(const mi_tensor & a, const mi_tensor & b) {
+    return a.data == b.data && a.type == b.type && same_shape(a, b) && (nrows(a) <= 1 || a.nb[1] == b.nb[1]);
+}
+
+static int lora_desc(const mi_tensor * x, const mi_tensor * a, const mi_tensor * b, LoraArgs & l) {
+    MI_TRY(check(x));
+    MI_TRY(check(a));
+    MI_TRY(check(b));
+    if (x->type != MI_TYPE_F32 || a->type != b->type || (a->type != MI_TYPE_BF16 && a->type != MI_TYPE_F16)) {
+        return MI_ERR_TYPE;
+    }
+    const int64_t k = a->ne[0], r = a->ne[1], n_ad = a->ne[2];
+    if (x->ne[0] != k || !uniform_rows(*x) || a->ne[3] != 1 || b->ne[3] != 1 || b->ne[0] != r || b->ne[2] != n_ad ||
+        k <= 0 || k % 32 != 0 || r <= 0) {
+        return MI_ERR_SHAPE;
+    }
+    const int64_t m = nrows(*x), n = b->ne[1];
+    if (r > 256 || (m + 15) / 16 * ((n + 63) / 64) >= kMaxRows || (n + 63) / 64 > 65535) {
+        return MI_ERR_UNSUPPORTED;
+    }
+    l      = LoraArgs{};
+    l.x    = (const char *) x->data;
+    l.x1   = (int64_t) x->nb[1];
+    l.a    = (const char *) a->data;
+    l.a1   = (int64_t) a->nb[1];
+    l.a2   = (int64_t) a->nb[2];
+    l.b    = (const char *) b->data;
+    l.b1   = (int64_t) b->nb[1];
+    l.b2   = (int64_t) b->nb[2];
+    l.m    = (uint32_t) m;
+    l.k    = (uint32_t) k;
+    l.n    = (uint32_t) n;
+    l.r    = (uint32_t) r;
+    l.n_ad = (int32_t) n_ad;
+    lora_plan(l);
+    return MI_OK;
+}
+
+int mi_lora_add_workspace(const mi_tensor * x, const mi_tensor * a, const mi_tensor * b, size_t * bytes) {
+    if (!bytes) {
+        return MI_ERR_NULL;
+    }
+    LoraArgs l;
+    MI_TRY(lora_desc(x, a, b, l));
+    *bytes = lora_workspace(l);
+    return MI_OK;
+}
+
+int mi_lora_add(const mi_tensor * y0, const mi_tensor * x, const mi_tensor * a, const mi_tensor * b,
+                const mi_tensor * ids, const mi_tensor * scales, const mi_tensor * y, void * workspace,
+                size_t workspace_bytes, int32_t * d_err, mi_stream stream) {
+    LoraArgs l;
+    MI_TRY(lora_desc(x, a, b, l));
+    MI_TRY(check(y0));
+    MI_TRY(check(y));
+    if (y0->type != MI_TYPE_F32 || y->type != MI_TYPE_F32) {
+        return MI_ERR_TYPE;
+    }
+    if (y0->ne[0] != l.n || nrows(*y0) != l.m || !uniform_rows(*y0) || y->ne[0] != l.n || nrows(*y) != l.m ||
+        !uniform_rows(*y)) {
+        return MI_ERR_SHAPE;
+    }
+    MI_TRY(check_i32(ids, l.m, false));
+    if (ids->nb[0] % 4 != 0) {
+        return MI_ERR_ALIGN;
+    }
+    if (scales) {
+        MI_TRY(check_vec(scales, l.n_ad));
+    }
+    if (!aligned(d_err, 4)) {
+        return MI_ERR_ALIGN;
+    }
+    if (l.m == 0 || l.n == 0) {
+        return MI_OK;
+    }
+    // a row's products read its x and y0 while other workgroups write y
+    if (views_overlap(*y, *x) || (views_overlap(*y, *y0) && !(y->data == y0->data && (l.m <= 1 || y->nb[1] == y0->nb[1])))) {
+        return MI_ERR_PARAM;
+    }
+    if (!workspace || workspace_bytes < lora_workspace(l)) {
+        return MI_ERR_PARAM;
+    }
+    if (!aligned(workspace, 16)) {
+        return MI_ERR_ALIGN;
+    }
+    l.ids    = (const char *) ids->data;
+    l.i0     = (int64_t) ids->nb[0];
+    l.scales = scales ? (const char *) scales->data : nullptr;
+    l.s0     = 4;
+    l.y0     = (const char *) y0->data;
+    l.y01    = (int64_t) y0->nb[1];
+    l.y      = (char *) y->data;
+    l.y1     = (int64_t) y->nb[1];
+    l.d_err  = d_err;
+    l.h      = (float *) workspace;
+    return finish(launch_lora(l, a->type, (hipStream_t) stream));
+}
+
+int mi_logits_adjust(const mi_tensor * logits, const mi_tensor * history, const mi_tensor * lengths,
+                     const mi_tensor * penalties, const mi_tensor * bias, const mi_tensor * allowed,
+                     const mi_tensor * state, const mi_tensor * y, int32_t * d_err, mi_stream stream) {
+    MI_TRY(check_act(logits));
+    MI_TRY(check_act(y));
+    if (y->type != logits->type) {
+        return MI_ERR_TYPE;
+    }
+    const int64_t V = logits->ne[0], rows = logits->ne[1];
+    if (!same_shape(*logits, *y) || logits->ne[2] != 1 || logits->ne[3] != 1) {
+        return MI_ERR_SHAPE;
+    }
+    if ((history != nullptr) != (penalties != nullptr) || (lengths && !history) || (state && !allowed)) {
+        return MI_ERR_NULL;
+    }
+    LogitsArgs a{};
+    a.x       = (const char *) logits->data;
+    a.x1      = (int64_t) logits->nb[1];
+    a.y       = (char *) y->data;
+    a.y1      = (int64_t) y->nb[1];
+    a.rows    = (uint32_t) rows;
+    a.n_vocab = V;
+    if (history) {
+        MI_TRY(check(history));
+        MI_TRY(check(penalties));
+        if (history->type != MI_TYPE_I32 || penalties->type != MI_TYPE_F32) {
+            return MI_ERR_TYPE;
+        }
+        if (history->ne[1] != rows || history->ne[2] != 1 || history->ne[3] != 1 || penalties->ne[0] != 3 ||
+            penalties->ne[1] != rows || penalties->ne[2] != 1 || penalties->ne[3] != 1) {
+            return MI_ERR_SHAPE;
+        }
+        if (lengths) {
+            MI_TRY(check_i32(lengths, rows, false));
+            a.len = (const char *) lengths->data;
+            a.l0  = (int64_t) lengths->nb[0];
+        }
+        if (history->ne[0] > 0) {  // no token at all: nothing to count
+            a.hist   = (const char *) history->data;
+            a.h1     = (int64_t) history->nb[1];
+            a.n_hist = (int32_t) history->ne[0];
+            a.pen    = (const char *) penalties->data;
+            a.p1     = (int64_t) penalties->nb[1];
+        }
+    }
+    if (bias) {
+        MI_TRY(check(bias));
+        if (bias->type != MI_TYPE_F32) {
+            return MI_ERR_TYPE;
+        }
+        if (bias->ne[0] != V || (bias->ne[1] != 1 && bias->ne[1] != rows) || bias->ne[2] != 1 || bias->ne[3] != 1) {
+            return MI_ERR_SHAPE;
+        }
+        a.bias = (const char *) bias->data;
+        a.b1   = bias->ne[1] == 1 ? 0 : (int64_t) bias->nb[1];
+    }
+    if (allowed) {
+        MI_TRY(check(allowed));
+        if (allowed->type != MI_TYPE_I32) {
+            return MI_ERR_TYPE;
+        }
+        if (allowed->ne[0] != (V + 31) / 32 || allowed->ne[2] != 1 || allowed->ne[3] != 1 ||
+            (!state && allowed->ne[1] != 1 && allowed->ne[1] != rows)) {
+            return MI_ERR_SHAPE;
+        }
+        a.allowed  = (const char *) allowed->data;
+        a.m1       = (int64_t) allowed->nb[1];
+        a.n_states = (int32_t) allowed->ne[1];
+        if (state) {
+            MI_TRY(check_i32(state, rows, false));
+            a.state = (const char *) state->data;
+            a.st0   = (int64_t) state->nb[0];
+        }
+    }
+    for (const mi_tensor * t : { lengths, state }) {
+        if (t && t->nb[0] % 4 != 0) {
+            return MI_ERR_ALIGN;
+        }
+    }
+    if (!aligned(d_err, 4)) {
+        return MI_ERR_ALIGN;
+    }
+    if (rows > 65535) {
+        return MI_ERR_UNSUPPORTED;  // a grid's second dimension
+    }
+    if (V == 0 || rows == 0) {
+        return MI_OK;
+    }
+    if (views_overlap(*logits, *y) && !same_view(*logits, *y)) {
+        return MI_ERR_PARAM;
+    }
+    a.d_err = d_err;
+    return finish(launch_logits(a, logits->type, (hipStream_t) stream));
+}
+
 int mi_apg_buffer_bytes(const mi_tensor * cond, size_t * bytes) {
     if (!bytes) {
         return MI_ERR_NULL;

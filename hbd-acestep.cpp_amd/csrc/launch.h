@@ -228,6 +228,59 @@ void   mul_mat_q8_0_bind(MmvArgs & a, char * ws);
 int    launch_mul_mat_q8_0(const MmvArgs & a, hipStream_t s);
 int    launch_q8_0_repack(const char * src, int64_t nb1, uint32_t k, uint32_t n, char * dst, hipStream_t s);
 
+// ---- lora.hip ----------------------------------------------------------------
+// y = y0 + scale B (A x) with each row's own adapter (byte strides)
+struct LoraArgs {
+    const char * x;        // F32 [k, m]: rows at x1
+    int64_t      x1;
+    const char * a;        // [k, r, n_ad]: ranks at a1, adapters at a2
+    int64_t      a1, a2;
+    const char * b;        // [r, n, n_ad]: columns of y at b1, adapters at b2
+    int64_t      b1, b2;
+    const char * ids;      // I32 [m], at i0
+    int64_t      i0;
+    const char * scales;   // F32 [n_ad] at s0, or nullptr
+    int64_t      s0;
+    const char * y0;       // F32 [n, m]
+    int64_t      y01;
+    char *       y;
+    int64_t      y1;
+    int32_t *    d_err;
+    uint32_t     m, k, n, r;
+    int32_t      n_ad;
+    uint32_t     rp, ks, kstep, slots;  // from lora_plan
+    float *      h;        // workspace: [ks][m][rp]
+};
+void   lora_plan(LoraArgs & a);
+size_t lora_workspace(const LoraArgs & a);
+int    launch_lora(const LoraArgs & a, int type, hipStream_t s);
+
+// ---- logits.hip --------------------------------------------------------------
+struct LogitsArgs {
+    const char * x;        // [n_vocab, rows], rows at x1
+    int64_t      x1;
+    char *       y;
+    int64_t      y1;
+    uint32_t     rows;
+    int64_t      n_vocab;
+    const char * hist;     // I32 [n_hist, rows] at h1, or nullptr
+    int64_t      h1;
+    int32_t      n_hist;
+    const char * len;      // I32 [rows] at l0, or nullptr
+    int64_t      l0;
+    const char * pen;      // F32 [3, rows] at p1 (with hist)
+    int64_t      p1;
+    const char * bias;     // F32 [n_vocab, rows] at b1 (0: one for all), or nullptr
+    int64_t      b1;
+    const char * allowed;  // I32 [words, n_states] at m1, or nullptr
+    int64_t      m1;
+    int32_t      n_states;
+    const char * state;    // I32 [rows] at st0, or nullptr
+    int64_t      st0;
+    int32_t *    d_err;
+};
+int launch_logits(const LogitsArgs & a, int type, hipStream_t s);
+
 // ---- sampler.hip -----------------------------------------------------------
 struct ApgArgs {
     const float * cond;    // F32 [n][t][oc]

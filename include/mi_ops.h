@@ -387,6 +387,50 @@ int mi_mul_mat_q8_0_adaln(const void * w, int64_t k, int64_t n, const mi_tensor 
                           const mi_tensor * shift, float eps, const mi_tensor * sum, const mi_tensor * y,
                           void * workspace, size_t workspace_bytes, mi_stream stream);
 
+/* Low-rank adapters of many requests beside a shared projection, for rows whose
+ * requests each bring their own (the reference merges one adapter into the weights
+ * at load, adapter-merge.h; merged weights serve one adapter at a time):
+ *   y[:, t] = y0[:, t] + scales[id] * B[id] (A[id] x[:, t]),  id = ids[t]
+ *   x:     F32 [k, m...], k a multiple of 32, rows uniformly strided (the
+ *          projection's x); y0, y: F32 [n, m...] (the projection's y; y may be y0,
+ *          else they must not overlap; y must not overlap x: MI_ERR_PARAM)
+ *   a, b:  [k, r, n_adapters] and [r, n, n_adapters], both BF16 or both F16, r <= 256;
+ *          adapters of a lower rank are padded with zeros
+ *   ids:   I32 [m]; a negative id is a row without an adapter, y = y0; an id past the
+ *          last adapter is taken as one and counted in *d_err when d_err != NULL
+ *   scales: F32 [n_adapters] or NULL (1)
+ * Products and sums keep fp32 accuracy (x and A x as three bf16 parts each on the
+ * matrix cores). workspace: device memory of at least mi_lora_add_workspace() bytes,
+ * 16-byte aligned; calls that share one race. The size depends on the shapes and on
+ * the current device's CU count. */
+int mi_lora_add_workspace(const mi_tensor * x, const mi_tensor * a, const mi_tensor * b, size_t * bytes);
+int mi_lora_add(const mi_tensor * y0, const mi_tensor * x, const mi_tensor * a, const mi_tensor * b,
+                const mi_tensor * ids, const mi_tensor * scales, const mi_tensor * y, void * workspace,
+                size_t workspace_bytes, int32_t * d_err, mi_stream stream);
+
+/* Logits before a token is drawn: penalties for tokens that the row's history holds,
+ * a bias and a grammar's mask, for the host loop's constrained decoding
+ * (metadata-fsm.h; pipeline-lm.cpp:471) without reading the logits back. With c the
+ * times a token is in the row's history:
+ *   l' = c > 0 ? (l > 0 ? l / rep : l * rep) - c * freq - pres : l
+ *   y  = allowed ? l' + bias : -inf
+ * in fp32, in that order, rounded once to y's type.
+ *   logits, y: [n_vocab, rows], one type (F32/BF16/F16); y may be logits, else they must
+ *              not overlap (MI_ERR_PARAM)
+ *   history:   I32 [n, rows] or NULL; lengths: I32 [rows] or NULL (all n): row r's tokens
+ *              are the first lengths[r] (taken into [0, n]); tokens outside [0, n_vocab) are
+ *              skipped and counted in *d_err when d_err != NULL
+ *   penalties: F32 [3, rows], (rep, freq, pres) of each row; given exactly with history
+ *   bias:      F32 [n_vocab] or [n_vocab, rows], or NULL
+ *   allowed:   I32 [ceil(n_vocab / 32), n_states] or NULL: bit v % 32 of word v / 32 is set where
+ *              a state of the grammar allows token v; state: I32 [rows], each row's state
+ *              (negative: no grammar; past the last: none, and counted in *d_err), or NULL
+ *              (n_states 1: the same for all rows; n_states = rows: row r's own)
+ * A row whose state allows nothing is all -inf. */
+int mi_logits_adjust(const mi_tensor * logits, const mi_tensor * history, const mi_tensor * lengths,
+                     const mi_tensor * penalties, const mi_tensor * bias, const mi_tensor * allowed,
+                     const mi_tensor * state, const mi_tensor * y, int32_t * d_err, mi_stream stream);
+
 /* The DiT sampler's per-step math on the device (dit_ggml_generate,
  * dit-sampler.h:408-640), so the latents stay resident across steps.
  * Latents and velocities are F32 [Oc, T, N], contiguous.
