@@ -5,9 +5,12 @@
 // with k, v = (level - 8) d per block of 32 elements. Unlike a Q8_0 cache's, the
 // products take q as it is: a level has 4 bits, exact in fp16, so the matrix cores
 // multiply levels by q in fp16 and the block's d is applied to the fp32 sum.
-//  q      each row is scaled by a power of two so that its largest element is near
-//         2^13, then held as one fp16 (BF16 and F16 q, exact but for elements 2^-24
-//         of the row's largest) or as a high and a low one (F32 q, 22 bits).
+//  q      each row is scaled by a power of two so that its largest element lies in
+//         [2^10, 2^11). BF16 y: held as one fp16 (BF16 q: exact but for elements under
+//         2^-24 of the largest). F32 y: as a whole number and an fp16 remainder, 23 bits
+//         of the row's largest; the matrix cores' sums of whole numbers are exact, where
+//         sums of 24-bit terms are cut at each step (measured over the LM's decode size:
+//         y off by 4.1e-6 with two fp16 of any size, 2-norm over 2-norm, torch's fp32 6e-7).
 //  levels as fp16 operands are the nibbles themselves: 0x000n is n 2^-24 and 0x00n0
 //         16 n 2^-24, subnormals that the matrix cores take as they are, so two
 //         ANDs and a shift per pair make an operand; q's elements that meet a high
@@ -132,10 +135,11 @@ template <int D> struct Fa4 {
     static __device__ __forceinline__ int voff(int key) { return key * KROW + key / RPP * 16; }
 };
 
-// MS: 0 no mask, 1 one mask row for all rows of the tile, 2 a mask row each
-template <int D, int QP, bool OS, int MS, int W>
+// OS: F32 y (parts of q, P and V); MS: 0 no mask, 1 one mask row for all rows of the tile, 2 a mask row each
+template <int D, bool OS, int MS, int W>
 __global__ void __launch_bounds__(64 * W) k_fa4_dec(const FaArgs a) {
     using F           = Fa4<D>;
+    constexpr int QP  = OS ? 2 : 1;
     constexpr int NB  = F::NB, TK = F::TK, IPL = F::IPL, MT = F::MT;
     constexpr int MSB = MS == 1 ? F::MB * TK * 4 : 0;
     constexpr int WB  = F::WAVE + MSB;
@@ -194,34 +198,37 @@ __global__ void __launch_bounds__(64 * W) k_fa4_dec(const FaArgs a) {
     qmax     = fmaxf(qmax, __shfl_xor(qmax, 16, 64));
     qmax     = fmaxf(qmax, __shfl_xor(qmax, 32, 64));
     int ex   = (int) (__float_as_uint(qmax) >> 23) - 127;  // 2^ex <= qmax < 2^(ex + 1)
-    ex       = ex < -100 ? -100 : ex > 127 ? 13 : ex;      // a row that is not finite: as it is
-    const float up = __uint_as_float((uint32_t) (127 + 13 - ex) << 23);
-    const float qs = a.scale * FA4_LOG2E * __uint_as_float((uint32_t) (127 - 13 + ex) << 23);
+    ex       = ex < -100 ? -100 : ex > 127 ? 10 : ex;      // a row that is not finite: as it is
+    const float up = __uint_as_float((uint32_t) (127 + 10 - ex) << 23);
+    const float qs = a.scale * FA4_LOG2E * __uint_as_float((uint32_t) (127 - 10 + ex) << 23);
     fa4_h8      qb[QP][NB];
-    float       c0[NB];
+    float       c0[QP][NB];
 #pragma unroll
     for (int blk = 0; blk < NB; ++blk) {
-        float s[8], sum = 0.0f;
+        float s[8], sum[QP] = {};
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             qv[blk][e] *= up;
         }
-        fa4_slots(qv[blk], s);
+        float part[8], rest[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const _Float16 hi = (_Float16) s[e];
-            qb[0][blk][e]     = hi;
-            float used        = (float) hi;
-            if constexpr (QP == 2) {
-                const _Float16 lo = (_Float16) (s[e] - (float) hi);
-                qb[1][blk][e]     = lo;
-                used += (float) lo;
-            }
-            sum += e & 2 ? used * 16.0f : used;  // slots 2, 3, 6, 7 meet 16 times the level
+            part[e] = QP == 2 ? __builtin_rintf(qv[blk][e]) : qv[blk][e];
+            rest[e] = qv[blk][e] - part[e];
         }
-        sum += __shfl_xor(sum, 16, 64);
-        sum += __shfl_xor(sum, 32, 64);
-        c0[blk] = sum * (-8.0f / 16777216.0f);
+#pragma unroll
+        for (int p = 0; p < QP; ++p) {
+            fa4_slots(p ? rest : part, s);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                qb[p][blk][e] = (_Float16) s[e];
+                // slots 2, 3, 6, 7 meet 16 times the level
+                sum[p] += (float) qb[p][blk][e] * (e & 2 ? 16.0f : 1.0f);
+            }
+            sum[p] += __shfl_xor(sum[p], 16, 64);
+            sum[p] += __shfl_xor(sum[p], 32, 64);
+            c0[p][blk] = sum[p] * (-8.0f / 16777216.0f);
+        }
     }
 
     float  m = -INFINITY, l = 0.0f;
@@ -358,16 +365,16 @@ __global__ void __launch_bounds__(64 * W) k_fa4_dec(const FaArgs a) {
                 fa4_f4 t = { 0.0f, 0.0f, 0.0f, 0.0f };
 #pragma unroll
                 for (int blk = 0; blk < NB; ++blk) {
-                    const fa4_h8 x   = fa4_levels(kw[blk]);
-                    fa4_f4       acc = { c0[blk], c0[blk], c0[blk], c0[blk] };
-#pragma unroll
-                    for (int p = 0; p < QP; ++p) {
-                        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, qb[p][blk], acc, 0, 0, 0);
-                    }
+                    const fa4_h8 x  = fa4_levels(kw[blk]);
                     const fa4_f4 dk = *(const fa4_f4 *) (dkl + blk * F::DS + 16 * mt + 4 * q4);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        t[r] = __builtin_fmaf(acc[r], dk[r], t[r]);
+                    for (int p = QP - 1; p >= 0; --p) {
+                        const float  c   = c0[p][blk];
+                        const fa4_f4 acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, qb[p][blk], fa4_f4{ c, c, c, c }, 0, 0, 0);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            t[r] = __builtin_fmaf(acc[r], dk[r], t[r]);
+                        }
                     }
                 }
 #pragma unroll
@@ -606,15 +613,15 @@ size_t flash_attn_q4_workspace(const FaArgs & a, int D) {
     return a.splits > 1 ? (size_t) a.splits * a.nb * a.nkv * a.rows * (D + 4) * sizeof(float) : 0;
 }
 
-template <int D, int QP, bool OS>
+template <int D, bool OS>
 static void launch_dec(const FaArgs & a, hipStream_t s) {
     const dim3 grid((uint32_t) ((int64_t) a.nb * a.nkv * a.rblocks * a.splits)), wg(64 * FA4_W);
     if (a.mask == nullptr) {
-        MI_LAUNCH((k_fa4_dec<D, QP, OS, 0, FA4_W>), grid, wg, 0, s, a);
+        MI_LAUNCH((k_fa4_dec<D, OS, 0, FA4_W>), grid, wg, 0, s, a);
     } else if (a.n_q == 1 && a.mne2 == 1) {
-        MI_LAUNCH((k_fa4_dec<D, QP, OS, 1, FA4_W>), grid, wg, 0, s, a);
+        MI_LAUNCH((k_fa4_dec<D, OS, 1, FA4_W>), grid, wg, 0, s, a);
     } else {
-        MI_LAUNCH((k_fa4_dec<D, QP, OS, 2, FA4_W>), grid, wg, 0, s, a);
+        MI_LAUNCH((k_fa4_dec<D, OS, 2, FA4_W>), grid, wg, 0, s, a);
     }
     if (a.splits > 1) {
         MI_LAUNCH((k_fa4_combine<D>), dim3((uint32_t) (a.nb * a.nkv * a.rows)), dim3(64), 0, s, a);
@@ -624,11 +631,9 @@ static void launch_dec(const FaArgs & a, hipStream_t s) {
 template <int D>
 static int launch_d(const FaArgs & a, hipStream_t s) {
     if (a.ty == MI_TYPE_BF16) {
-        launch_dec<D, 1, false>(a, s);
-    } else if (a.tq == MI_TYPE_F32) {
-        launch_dec<D, 2, true>(a, s);
+        launch_dec<D, false>(a, s);
     } else {
-        launch_dec<D, 1, true>(a, s);
+        launch_dec<D, true>(a, s);
     }
     return MI_OK;
 }

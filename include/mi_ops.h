@@ -255,7 +255,7 @@ int mi_timestep_embedding(const mi_tensor * t, int dim, int max_period, const mi
  * be 0 (the only values the reference passes); others return
  * MI_ERR_UNSUPPORTED. q is converted to K's dot type as ggml-cpu converts it
  * (fp16, bf16, or Q8_0 with the x86 rounding; with Q4_0 K it is used as it is,
- * to 22 bits of an F32 row's largest element); keys whose mask is -inf do not
+ * to 23 bits of an F32 row's largest element); keys whose mask is -inf do not
  * contribute; a row whose keys are all masked is NaN. The decode and split
  * kernels never read masked keys; the matrix-core prefill kernel (64 or more
  * (query, head) rows per KV head, D = 128) reads the K/V rows of keys masked

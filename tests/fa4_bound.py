@@ -4,7 +4,7 @@ arithmetic may be from it, element by element.
 With s the scores, p = exp(s - max s), L = sum p, and u = 2^-24:
   scores  A_j = scale sum_b |d_b| sum_e (level_e + 8) |q_e| bounds the terms of the two
           sums that make s_j (levels 0..15 and -8 sum q), 33 terms a block: 64 u A_j;
-          q held to 22 bits: 2^-22 A_j; the scaling by d, the sum over blocks, the row's
+          q held to 23 bits of the row's largest element: scale sum |k| max|q| 2^-23; the scaling by d, the sum over blocks, the row's
           scale and the mask's addition: 16 u A_j + 4 u |mask_j|
   p       2^-22 for the exponential, 2 u |s_j - max s| for its argument, and the score's
           error, doubled for the second order: rho_j
@@ -36,7 +36,7 @@ def row(q, k, v, mask, scale, f32_y):
     level = np.where(d > 0, np.abs(kf) / np.where(d > 0, d, 1) + 16, 16)  # |level - 8| + 16 >= level + 8
     s = kf @ q * scale
     A = (d * level) @ np.abs(q) * abs(scale)
-    ds = (2.0 ** -22 + 80 * U) * A
+    ds = 80 * U * A + 2.0 ** -23 * np.abs(kf).sum(1) * np.abs(q).max() * abs(scale)
     if mask is not None:
         s = s + mask
         ds = ds + 4 * U * np.abs(mask)
