@@ -2384,6 +2384,12 @@ static int launch_k(const FaArgs & a, int D, hipStream_t s) {
     }
 }
 
+void launch_fa_mask_summary(const FaArgs & a, hipStream_t s) {
+    MI_LAUNCH(k_fa_mask_summary, dim3((uint32_t) (((a.n_kv + 63) / 64 + FA_SUM_T - 1) / FA_SUM_T), (uint32_t) a.ngq,
+                                               (uint32_t) (a.mne3 * a.mne2)),
+                       dim3(64), 0, s, a);
+}
+
 int launch_flash_attn(const FaArgs & a, int kt, int D, hipStream_t s) {
     if (kt == MI_TYPE_Q4_0) {
         return launch_flash_attn_q4(a, D, s);
@@ -2393,10 +2399,7 @@ int launch_flash_attn(const FaArgs & a, int kt, int D, hipStream_t s) {
     }
     if (a.mfma) {
         if (a.msum != nullptr) {
-            MI_LAUNCH(k_fa_mask_summary, dim3((uint32_t) (((a.n_kv + 63) / 64 + FA_SUM_T - 1) / FA_SUM_T),
-                                                       (uint32_t) a.ngq,
-                                                       (uint32_t) (a.mne3 * a.mne2)),
-                               dim3(64), 0, s, a);
+            launch_fa_mask_summary(a, s);
         }
         const dim3 grid((uint32_t) (a.tfull + 2 * a.tsplit));
         if (kt == MI_TYPE_Q8_0) {

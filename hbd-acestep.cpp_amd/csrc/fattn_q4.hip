@@ -29,6 +29,10 @@ typedef _Float16 fa4_h8 __attribute__((ext_vector_type(8)));
 typedef float    fa4_f4 __attribute__((ext_vector_type(4)));
 typedef int      fa4_v2i __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) fa4_v2i fa4_lds_v2i;
+typedef short fa4_v4s __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) fa4_v4s fa4_lds_v4s;
+typedef float    fa4_f4u __attribute__((ext_vector_type(4), aligned(4)));  // y at its element's alignment
+typedef uint32_t fa4_u2u __attribute__((ext_vector_type(2), aligned(2)));
 typedef uint32_t fa4_u4 __attribute__((ext_vector_type(4), aligned(4)));  // rows are 4-byte aligned
 
 constexpr float FA4_LOG2E = 1.44269504088896340736f;
@@ -584,39 +588,572 @@ __global__ void __launch_bounds__(64) k_fa4_combine(const FaArgs a) {
     }
 }
 
-constexpr int FA4_W = 4;  // waves per workgroup
+// Many query rows: a workgroup of W waves owns W * 16 * RT rows (query position, head) of
+// one KV head and walks the keys in tiles of T, K and V dequantized once per tile into LDS,
+// double-buffered, the next tile's raw blocks in flight. A wave holds RT tiles of 16 rows;
+// the products are those of k_fa4_dec (S^T = K Q^T, O^T = V^T P^T, 16x16x32), their A
+// operands read from LDS once for all RT tiles.
+//  K      BF16 y: (level - 8) d in fp16, one rounding (2^-11 of each term of q . k, where q
+//         itself has 8 bits), so that the sum over blocks stays in the accumulator; F32 y: the
+//         levels as whole numbers, the sums of each block scaled by d as in k_fa4_dec
+//  V      (level - 8) d in fp16, F32 y: a high and a low part
+//  order  a block's 32 elements lie in LDS as (half, group of 4, 0 2 1 3), the order in which
+//         masks and shifts unpack the nibbles; q is read in the same order, and the output
+//         lane's 4 values are one group of 4, put back when they are stored
+// Tiles in which a d leaves fp16's range, or a V block is not finite while some key is masked,
+// are found when they are staged and staged again (d / 16 with P or the scores * 16; v = 0
+// for keys that no row of the workgroup attends to).
+// The maximum that p refers to moves only when a row's grows by more than 2^3, so most tiles
+// need no reduction over lanes. Masks are looked up per tile in k_fa_mask_summary's bytes.
+template <int D, bool OS> struct Fa4P {
+    static constexpr int NB = D / 32;
+    static constexpr int T  = D == 256 ? 32 : 64;       // keys per tile
+    static constexpr int RT = D == 256 ? 1 : 2;         // row tiles per wave
+    static constexpr int W  = D == 256 || (OS && D == 128) ? 8 : 4;
+    static constexpr int BQ = W * 16 * RT;
+    static constexpr int KS = D * 2 + 16;               // K row stride: 16 keys on distinct banks
+    static constexpr int VS = D * 2 + 32;               // V row stride: 8 keys on distinct banks, transposed reads
+    static constexpr int VP = OS ? 2 : 1;
+    static constexpr int DS = T + 16;                   // entries per block in the table of K's d (F32 y)
+    static constexpr int KB = T * KS;
+    static constexpr int VB = T * VS;
+    static constexpr int DB = OS ? NB * DS * 4 : 0;
+    static constexpr int BUF = KB + VP * VB + DB;
+    static constexpr int CH  = 2048;                    // tiles whose mask flags are held at once
+};
+
+__device__ __forceinline__ float fa4_max_groups(float v) {  // over the 4 lane groups of 16
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v            = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    const auto t = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(t[0]), __uint_as_float(t[1]));
+}
+
+template <int D, bool OS, bool MSK>
+__global__ void __launch_bounds__((64 * Fa4P<D, OS>::W)) __attribute__((amdgpu_waves_per_eu(2)))
+k_fa4_pre(const FaArgs a) {
+    using F          = Fa4P<D, OS>;
+    constexpr int NB = F::NB, T = F::T, RT = F::RT, W = F::W, MT = T / 16, QP = OS ? 2 : 1;
+    constexpr int NI = 2 * T * NB;                       // blocks per tile, K's then V's
+    constexpr int IT = (NI + 64 * W - 1) / (64 * W);     // per thread
+    __shared__ __align__(16) char lds[2 * F::BUF];
+    __shared__ uint32_t           tflag[2][W];           // 1: V's d past fp16, 2: K's, 4: V not finite
+    __shared__ uint64_t           lvw[W];
+    __shared__ uint8_t            cfl[MSK ? F::CH : 1];  // 1: a live key, 2: a value that is not 0
+
+    const int      tid = threadIdx.x, lane = tid & 63;
+    const int      wv  = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int      c16 = lane & 15, q4 = lane >> 4;
+    const uint32_t item  = blockIdx.x / (uint32_t) a.splits;
+    const uint32_t split = blockIdx.x - item * (uint32_t) a.splits;
+    const uint32_t nbg   = (uint32_t) (a.nb * a.nkv);
+    const uint32_t bg    = item % nbg;
+    const int      r0    = (a.rblocks - 1 - (int) (item / nbg)) * F::BQ;  // last rows first: the longest under a causal mask
+    const uint32_t b     = bg / (uint32_t) a.nkv;
+    const uint32_t g     = bg - b * (uint32_t) a.nkv;
+    const uint32_t kb    = b / (uint32_t) a.rk3;
+    const char *   kg    = a.k + (int64_t) kb * a.k3 + (int64_t) g * a.k2;
+    const char *   vg    = a.v + (int64_t) kb * a.v3 + (int64_t) g * a.v2;
+
+    // q: row tile rt, lane (row c16, group q4): positions 8 q4 .. 8 q4 + 7 of each block
+    fa4_h8       qb[RT][QP][NB];
+    float        qs[RT];
+    const char * mrow[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const int r  = r0 + (wv * RT + rt) * 16 + c16;
+        const int rc = r < a.rows ? r : a.rows - 1;
+        const int iq = rc / a.rk, h = (int) g * a.rk + (rc - iq * a.rk);
+        if constexpr (MSK) {
+            mrow[rt] = a.mask + (int64_t) (b % (uint32_t) a.mne3) * a.m3 + (int64_t) (h % a.mne2) * a.m2 + (int64_t) iq * a.m1;
+        }
+        const char * qp = a.q + (int64_t) b * a.q3 + (int64_t) h * a.q2 + (int64_t) iq * a.q1;
+        float        qv[NB][8], qmax = 0.0f;
+#pragma unroll
+        for (int blk = 0; blk < NB; ++blk) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int i = blk * 32 + 16 * (q4 >> 1) + 8 * (q4 & 1) + (e & 4) + ((e & 1) << 1 | (e >> 1 & 1));
+                qv[blk][e]  = a.tq == MI_TYPE_F32    ? load_elem<MI_TYPE_F32>(qp + (size_t) i * 4)
+                              : a.tq == MI_TYPE_BF16 ? load_elem<MI_TYPE_BF16>(qp + (size_t) i * 2)
+                                                     : load_elem<MI_TYPE_F16>(qp + (size_t) i * 2);
+                qmax        = fmaxf(qmax, fabsf(qv[blk][e]));
+            }
+        }
+        qmax           = fa4_max_groups(qmax);
+        int ex         = (int) (__float_as_uint(qmax) >> 23) - 127;
+        ex             = ex < -100 ? -100 : ex > 127 ? 10 : ex;
+        const float up = __builtin_copysignf(__uint_as_float((uint32_t) (127 + 10 - ex) << 23), a.scale);
+        qs[rt]         = fabsf(a.scale) * FA4_LOG2E * __uint_as_float((uint32_t) (127 - 10 + ex) << 23);
+#pragma unroll
+        for (int blk = 0; blk < NB; ++blk) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float v = qv[blk][e] * up, w = OS ? __builtin_rintf(v) : v;
+                qb[rt][0][blk][e] = (_Float16) w;
+                if constexpr (OS) {
+                    qb[rt][1][blk][e] = (_Float16) (v - w);
+                }
+            }
+        }
+    }
+
+    float  m[RT], l[RT];
+    fa4_f4 o[RT][2 * NB];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        m[rt] = -INFINITY;
+        l[rt] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 2 * NB; ++i) {
+            o[rt][i] = fa4_f4{ 0.0f, 0.0f, 0.0f, 0.0f };
+        }
+    }
+
+    Fa4Raw raw[IT];
+    auto   load = [&](int t) {
+        const int t0 = t * T, last = a.n_kv - 1 - t0;
+#pragma unroll
+        for (int i = 0; i < IT; ++i) {
+            const int idx = i * 64 * W + tid;
+            if (NI % (64 * W) == 0 || idx < NI) {
+                const bool isv = idx >= T * NB;
+                const int  j = isv ? idx - T * NB : idx, blk = j % NB;
+                const int  key = j / NB < last ? j / NB : last;  // past the end: the last key again
+                raw[i]         = fa4_load((isv ? vg : kg) + (int64_t) (t0 + key) * (isv ? a.v1 : a.k1), blk);
+            }
+        }
+    };
+    // raw blocks -> buffer bf. fix: 1, 2: V's, K's d / 16; keys out of `live` as v = 0
+    auto stage = [&](int bf, uint32_t fix, uint64_t live) {
+        char *   kl = lds + bf * F::BUF, *vl = kl + F::KB;
+        float *  dl = (float *) (vl + F::VP * F::VB);
+        uint32_t fl = 0;
+#pragma unroll
+        for (int i = 0; i < IT; ++i) {
+            const int idx = i * 64 * W + tid;
+            if (NI % (64 * W) == 0 || idx < NI) {
+                const bool isv = idx >= T * NB;
+                const int  j = isv ? idx - T * NB : idx, blk = j % NB, key = j / NB;
+                float      d;
+                uint32_t   w[4];
+                fa4_block(raw[i], blk, d, w);
+                if (isv) {
+                    d = live >> key & 1 ? d : 0.0f;
+                    fl |= fabsf(d) <= FA4_BIG ? 0u : fabsf(d) <= 65504.0f ? 1u : 4u;
+                    d = fix & 1 ? d * 0.0625f : d;
+                } else if (!OS) {
+                    fl |= fabsf(d) > FA4_BIG && fabsf(d) <= 65504.0f ? 2u : 0u;
+                    d = fix & 2 ? d * 0.0625f : d;
+                } else {
+                    dl[blk * F::DS + key] = d;
+                }
+                const _Float16 dh = (_Float16) d;
+                const fa4_h2   dd = { dh, dh };
+                uint32_t       q[16], ql[16];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {  // low (0 2), low (1 3), high (0 2), high (1 3)
+                        const uint32_t x = k & 1 ? w[e] >> 8 : w[e];
+                        const fa4_h2   n = k & 2 ? fa4_high(x) : fa4_low(x), v = n * dd;
+                        const int      at = (k & 2) * 4 + 2 * e + (k & 1);
+                        q[at] = OS && !isv ? fa4_bits(n) : fa4_bits(v);
+                        if constexpr (OS) {
+                            ql[at] = fa4_bits(__builtin_elementwise_fma(n, dd, -v));
+                        }
+                    }
+                }
+                char * p = isv ? vl + key * F::VS + blk * 64 : kl + key * F::KS + blk * 64;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    *(uint4 *) (p + 16 * e) = make_uint4(q[4 * e], q[4 * e + 1], q[4 * e + 2], q[4 * e + 3]);
+                    if constexpr (OS) {
+                        if (isv) {
+                            *(uint4 *) (p + F::VB + 16 * e) = make_uint4(ql[4 * e], ql[4 * e + 1], ql[4 * e + 2], ql[4 * e + 3]);
+                        }
+                    }
+                }
+            }
+        }
+        fl = (__builtin_amdgcn_ballot_w64(fl & 1) ? 1u : 0u) | (__builtin_amdgcn_ballot_w64(fl & 2) ? 2u : 0u) |
+             (__builtin_amdgcn_ballot_w64(fl & 4) ? 4u : 0u);
+        if (lane == 0) {
+            tflag[bf][wv] = fl;
+        }
+    };
+
+    const int ntile = (a.n_kv + T - 1) / T;
+    const int tbeg  = (int) ((int64_t) ntile * split / a.splits), tend = (int) ((int64_t) ntile * (split + 1) / a.splits);
+    const int iq0 = r0 / a.rk, iq1 = (r0 + F::BQ < a.rows ? r0 + F::BQ - 1 : a.rows - 1) / a.rk;
+    for (int cb = tbeg; cb < tend; cb += F::CH) {
+        const int ce = tend - cb < F::CH ? tend : cb + F::CH;
+        if constexpr (MSK) {
+            const int nts = (a.n_kv + 63) / 64, nh = a.rk < a.mne2 ? a.rk : a.mne2;
+            __syncthreads();  // the chunk before is done with its flags
+            for (int t = cb + tid; t < ce; t += 64 * W) {
+                uint32_t f = 0;
+                for (int hh = 0; hh < nh; ++hh) {
+                    const int       mh = (int) (b % (uint32_t) a.mne3) * a.mne2 + ((int) g * a.rk + hh) % a.mne2;
+                    const uint8_t * mp = a.msum + ((int64_t) mh * a.ngq) * nts + t * T / 64;
+                    for (int gr = iq0 >> 4; gr <= iq1 >> 4; ++gr) {
+                        f |= mp[(int64_t) gr * nts];
+                    }
+                }
+                cfl[t - cb] = (uint8_t) f;
+            }
+            __syncthreads();
+        }
+        auto next = [&](int t) {  // the first tile from t on with a live key, or ce
+            if constexpr (MSK) {
+                while (t < ce) {
+                    const uint64_t v = __builtin_amdgcn_ballot_w64(t + lane < ce && (cfl[t + lane - cb < F::CH ? t + lane - cb : 0] & 1));
+                    if (v) {
+                        return t + (int) __builtin_ctzll(v);
+                    }
+                    t += 64;
+                }
+                return ce;
+            } else {
+                return t;
+            }
+        };
+        int t = next(cb);
+        if (t >= ce) {
+            continue;
+        }
+        load(t);
+        int bf = 0;
+        stage(0, 0, ~0ull);
+        int tn = next(t + 1);
+        if (tn < ce) {
+            load(tn);
+        }
+        __syncthreads();
+        while (true) {
+            if (tn < ce) {
+                stage(bf ^ 1, 0, ~0ull);
+            }
+            const int t2 = tn < ce ? next(tn + 1) : ce;
+            if (t2 < ce) {
+                load(t2);
+            }
+            const int    t0 = t * T;
+            const char * kl = lds + bf * F::BUF;
+            const char * vl = kl + F::KB;
+            const float * dl = (const float *) (vl + F::VP * F::VB);
+            const bool   clean = t0 + T <= a.n_kv && (!MSK || !(cfl[MSK ? t - cb : 0] & 2));
+            uint32_t     fl    = 0;
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                fl |= tflag[bf][w];
+            }
+            fl = __builtin_amdgcn_readfirstlane(fl);
+            float kf = 1.0f;  // what the scores are to be multiplied by
+            if (fl != 0) {
+                // some d past fp16, or a V block that is not finite: the tile again, scaled, without
+                // the keys that no row attends to
+                uint64_t live = 0;
+                if (!clean && (fl & 4)) {
+                    for (int rt = 0; rt < RT; ++rt) {
+                        for (int k = 0; k < T; k += 4) {
+                            const int  key = k + q4;
+                            bool       on = t0 + key < a.n_kv;
+                            if constexpr (MSK) {
+                                on = on && *(const uint16_t *) (mrow[rt] + (int64_t) (on ? t0 + key : 0) * 2) != 0xFC00u;
+                            }
+                            const uint64_t v = __builtin_amdgcn_ballot_w64(on);
+                            for (int gr = 0; gr < 4; ++gr) {
+                                live |= (uint64_t) ((v >> (16 * gr) & 0xffffu) != 0) << (k + gr);
+                            }
+                        }
+                    }
+                    if (lane == 0) {
+                        lvw[wv] = live;
+                    }
+                    __syncthreads();
+                    for (int w = 0; w < W; ++w) {
+                        live |= lvw[w];
+                    }
+                } else {
+                    live = ~0ull;
+                }
+                __syncthreads();  // every wave has read the tile's flags
+                load(t);
+                stage(bf, fl & 3, live);
+                if (t2 < ce) {
+                    load(t2);
+                }
+                __syncthreads();
+                kf = fl & 2 ? 16.0f : 1.0f;
+            }
+
+            fa4_f4 s[RT][MT];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                const char * kp = kl + (16 * mt + c16) * F::KS + q4 * 16;
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    s[rt][mt] = fa4_f4{ 0.0f, 0.0f, 0.0f, 0.0f };
+                }
+#pragma unroll
+                for (int blk = 0; blk < NB; ++blk) {
+                    const fa4_h8 x = *(const fa4_h8 *) (kp + blk * 64);
+                    if constexpr (OS) {
+                        const fa4_f4 dk = *(const fa4_f4 *) (dl + blk * F::DS + 16 * mt + 4 * q4);
+#pragma unroll
+                        for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+                            for (int p = 1; p >= 0; --p) {
+                                const fa4_f4 acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                                    x, qb[rt][OS ? p : 0][blk], fa4_f4{ 0.0f, 0.0f, 0.0f, 0.0f }, 0, 0, 0);
+#pragma unroll
+                                for (int r = 0; r < 4; ++r) {
+                                    s[rt][mt][r] = __builtin_fmaf(acc[r], dk[r], s[rt][mt][r]);
+                                }
+                            }
+                        }
+                    } else {
+#pragma unroll
+                        for (int rt = 0; rt < RT; ++rt) {
+                            s[rt][mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, qb[rt][0][blk], s[rt][mt], 0, 0, 0);
+                        }
+                    }
+                }
+            }
+            float fac[RT], lm[RT];
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                fac[rt] = qs[rt] * kf;
+            }
+            if (!clean) {  // scores with their mask values, in units of log2
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const int  key = t0 + 16 * mt + 4 * q4 + r;
+                            const bool in  = key < a.n_kv;
+                            float      mk  = in ? 0.0f : -INFINITY;
+                            if constexpr (MSK) {
+                                const float x = f16_lo(*(const uint16_t *) (mrow[rt] + (int64_t) (in ? key : a.n_kv - 1) * 2));
+                                mk            = in ? x * FA4_LOG2E : -INFINITY;
+                            }
+                            s[rt][mt][r] = mk == -INFINITY ? -INFINITY : __builtin_fmaf(s[rt][mt][r], fac[rt], mk);
+                        }
+                    }
+                    fac[rt] = 1.0f;
+                }
+            }
+            bool grow = false;
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                float x = -INFINITY;
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    x = fmaxf(fmaxf(x, s[rt][mt][0]), s[rt][mt][1]);
+                    x = fmaxf(fmaxf(x, s[rt][mt][2]), s[rt][mt][3]);
+                }
+                lm[rt] = x * fac[rt];
+                grow   = grow || lm[rt] > m[rt] + 3.0f;
+            }
+            if (__builtin_amdgcn_ballot_w64(grow) != 0) {
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    const float mn = fmaxf(m[rt], fa4_max_groups(lm[rt]));
+                    const float al = m[rt] == mn ? 1.0f : __builtin_amdgcn_exp2f(m[rt] - mn);
+                    m[rt]          = mn;
+                    l[rt] *= al;
+#pragma unroll
+                    for (int i = 0; i < 2 * NB; ++i) {
+                        o[rt][i] *= al;
+                    }
+                }
+            }
+            const float pf = fl & 1 ? 16.0f : 1.0f;
+            fa4_h8      ph[RT][T / 32], pl[OS ? RT : 1][T / 32];
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                const float mu = FA4_OFF - (m[rt] == -INFINITY ? 0.0f : m[rt]);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rt][mt][r], fac[rt], mu));
+                        l[rt] += p;
+                        s[rt][mt][r] = p;
+                    }
+                }
+                if (fl & 1) {
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) {
+                        s[rt][mt] *= pf;
+                    }
+                }
+#pragma unroll
+                for (int kk = 0; kk < T / 32; ++kk) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float    p = s[rt][2 * kk + e / 4][e & 3];
+                        const _Float16 h = (_Float16) p;
+                        ph[rt][kk][e]    = h;
+                        if constexpr (OS) {
+                            pl[rt][kk][e] = (_Float16) (p - (float) h);
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (int kk = 0; kk < T / 32; ++kk) {
+                // lane m of a group of 16 addresses key m / 4 of the group's 4, positions 4 (m % 4)
+                const char * vp = vl + (32 * kk + 4 * q4 + (c16 >> 2)) * F::VS + (c16 & 3) * 8;
+#pragma unroll
+                for (int dt = 0; dt < 2 * NB; ++dt) {
+                    fa4_h8 v[F::VP];
+#pragma unroll
+                    for (int p = 0; p < F::VP; ++p) {
+                        const fa4_v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((fa4_lds_v4s *) (vp + p * F::VB + dt * 32));
+                        const fa4_v4s z = __builtin_amdgcn_ds_read_tr16_b64_v4i16((fa4_lds_v4s *) (vp + p * F::VB + dt * 32 + 16 * F::VS));
+                        v[p] = __builtin_bit_cast(fa4_h8, __builtin_shufflevector(x, z, 0, 1, 2, 3, 4, 5, 6, 7));
+                    }
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) {
+                        fa4_f4 & oo = o[rt][dt];
+                        oo          = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[0], ph[rt][kk], oo, 0, 0, 0);
+                        if constexpr (OS) {
+                            oo = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[0], pl[rt][kk], oo, 0, 0, 0);
+                            oo = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[F::VP - 1], ph[rt][kk], oo, 0, 0, 0);
+                        }
+                    }
+                }
+            }
+            if (tn >= ce) {
+                break;
+            }
+            __syncthreads();
+            t  = tn;
+            tn = t2;
+            bf ^= 1;
+        }
+        __syncthreads();  // the next chunk stages into the buffers
+    }
+
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        float lr = l[rt];
+        lr += __shfl_xor(lr, 16, 64);
+        lr += __shfl_xor(lr, 32, 64);
+        const int r = r0 + (wv * RT + rt) * 16 + c16;
+        if (r >= a.rows) {
+            continue;
+        }
+        const int iq = r / a.rk, h = (int) g * a.rk + (r - iq * a.rk);
+        if (a.splits > 1) {
+            float * p = a.ws + (((int64_t) bg * a.rows + r) * a.splits + split) * (D + 4);
+            if (q4 == 0) {
+                p[0] = m[rt];
+                p[1] = lr;
+            }
+#pragma unroll
+            for (int dt = 0; dt < 2 * NB; ++dt) {
+                const fa4_f4 v = o[rt][dt];
+                *(float4 *) (p + 4 + dt * 16 + 4 * q4) = make_float4(v[0], v[2], v[1], v[3]);
+            }
+        } else {
+            char *      yp  = a.y + (int64_t) b * a.y3 + (int64_t) iq * a.y2 + (int64_t) h * a.y1;
+            const float inv = 1.0f / lr;  // no live key: 0 * inf
+#pragma unroll
+            for (int dt = 0; dt < 2 * NB; ++dt) {
+                const fa4_f4 v  = o[rt][dt] * inv;
+                const int    at = dt * 16 + 4 * q4;
+                if constexpr (OS) {
+                    *(fa4_f4u *) (yp + (size_t) at * 4) = fa4_f4u{ v[0], v[2], v[1], v[3] };
+                } else {
+                    *(fa4_u2u *) (yp + (size_t) at * 2) = fa4_u2u{ pack_bf16x2(v[0], v[2]), pack_bf16x2(v[1], v[3]) };
+                }
+            }
+        }
+    }
+}
+
+constexpr int FA4_W        = 4;   // waves per workgroup of the kernel for few rows
+constexpr int FA4_DEC_ROWS = 32;  // rows (query position, head) of a KV head that it takes
+
+// rows of a workgroup of the kernel for many rows
+static int fa4_bq(int D, bool f32) {
+    switch (D) {
+        case 64:
+            return f32 ? Fa4P<64, true>::BQ : Fa4P<64, false>::BQ;
+        case 128:
+            return f32 ? Fa4P<128, true>::BQ : Fa4P<128, false>::BQ;
+        default:
+            return f32 ? Fa4P<256, true>::BQ : Fa4P<256, false>::BQ;
+    }
+}
 
 void flash_attn_q4_plan(FaArgs & a, int D) {
     a.rows    = a.n_q * a.rk;
     a.rblocks = (a.rows + 15) / 16;
     a.splits  = 1;
-    const int     tk     = D == 256 ? 32 : 64;
-    const int64_t items  = (int64_t) a.nb * a.nkv * a.rblocks;
-    const int64_t tiles  = ((int64_t) a.n_kv + tk - 1) / tk;
-    if (items == 0 || tiles == 0) {
+    a.ngq     = (a.n_q + 15) / 16;
+    const int     tk    = D == 256 ? 32 : 64;
+    const int64_t tiles = ((int64_t) a.n_kv + tk - 1) / tk;
+    if (a.nb == 0 || a.rows == 0 || tiles == 0) {
         return;
     }
     if (a.n_kv > 1 << 27) {
         a.splits = 0;  // a wave's walk counts keys in 32 bits, 8 tiles of every wave ahead
         return;
     }
-    // enough waves for 16 per CU, at most one tile each
-    const int64_t want = ((int64_t) num_cus() * 16 / FA4_W + items - 1) / items;
-    const int64_t most = (tiles + FA4_W - 1) / FA4_W;
-    a.splits           = (int) (want < most ? want : most);
+    a.mfma = a.rows > FA4_DEC_ROWS && a.ngq <= 65535 && (int64_t) a.nb * a.nh <= 65535;
+    int64_t items, want, most;
+    if (a.mfma) {
+        // the workspace is sized without y: its type (rows per workgroup) must not change the splits
+        a.rblocks = (a.rows + 127) / 128;
+        items     = (int64_t) a.nb * a.nkv * a.rblocks;
+        want      = (int64_t) num_cus() * 2 / items;
+        most      = (tiles + 7) / 8;
+    } else {
+        items = (int64_t) a.nb * a.nkv * a.rblocks;
+        // enough waves for 16 per CU, at most one tile each
+        want = ((int64_t) num_cus() * 16 / FA4_W + items - 1) / items;
+        most = (tiles + FA4_W - 1) / FA4_W;
+    }
+    a.splits = (int) (want < 1 ? 1 : want < most ? want : most);
     if (items * a.splits >= ((int64_t) 1 << 31)) {
         a.splits = 0;  // more workgroups than a grid has
     }
+    if (a.mfma) {
+        const int bq = fa4_bq(D, a.ty == MI_TYPE_F32);
+        a.rblocks    = (a.rows + bq - 1) / bq;
+    }
+}
+
+// partial results of split keys, then the mask's summary bytes (for the largest mask a call may pass)
+static size_t fa4_parts(const FaArgs & a, int D) {
+    const size_t n = a.splits > 1 ? (size_t) a.splits * a.nb * a.nkv * a.rows * (D + 4) * sizeof(float) : 0;
+    return (n + 255) / 256 * 256;
 }
 
 size_t flash_attn_q4_workspace(const FaArgs & a, int D) {
-    return a.splits > 1 ? (size_t) a.splits * a.nb * a.nkv * a.rows * (D + 4) * sizeof(float) : 0;
+    return fa4_parts(a, D) + (a.mfma ? (size_t) a.nb * a.nh * a.ngq * ((a.n_kv + 63) / 64) : 0);
 }
 
 template <int D, bool OS>
 static void launch_dec(const FaArgs & a, hipStream_t s) {
     const dim3 grid((uint32_t) ((int64_t) a.nb * a.nkv * a.rblocks * a.splits)), wg(64 * FA4_W);
-    if (a.mask == nullptr) {
+    if (a.mfma) {
+        const dim3 wp(64 * Fa4P<D, OS>::W);
+        if (a.mask && a.n_kv > 0) {
+            FaArgs m = a;
+            m.msum   = (uint8_t *) a.ws + fa4_parts(a, D);
+            launch_fa_mask_summary(m, s);
+            MI_LAUNCH((k_fa4_pre<D, OS, true>), grid, wp, 0, s, m);
+        } else {
+            MI_LAUNCH((k_fa4_pre<D, OS, false>), grid, wp, 0, s, a);
+        }
+    } else if (a.mask == nullptr) {
         MI_LAUNCH((k_fa4_dec<D, OS, 0, FA4_W>), grid, wg, 0, s, a);
     } else if (a.n_q == 1 && a.mne2 == 1) {
         MI_LAUNCH((k_fa4_dec<D, OS, 1, FA4_W>), grid, wg, 0, s, a);

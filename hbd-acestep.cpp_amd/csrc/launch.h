@@ -177,6 +177,8 @@ void   flash_attn_plan(FaArgs & a, int D);
 size_t flash_attn_workspace(const FaArgs & a, int D);
 size_t flash_attn_part_offset(const FaArgs & a);
 int    launch_flash_attn(const FaArgs & a, int kt, int D, hipStream_t s);
+// one byte per (mask batch and head, 16 query positions, 64 keys) into a.msum
+void   launch_fa_mask_summary(const FaArgs & a, hipStream_t s);
 // Q4_0 K and V (fattn_q4.hip); the three above call these
 void   flash_attn_q4_plan(FaArgs & a, int D);
 size_t flash_attn_q4_workspace(const FaArgs & a, int D);

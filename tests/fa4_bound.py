@@ -6,6 +6,7 @@ With s the scores, p = exp(s - max s), L = sum p, and u = 2^-24:
           sums that make s_j (levels 0..15 and -8 sum q), 33 terms a block: 64 u A_j;
           q held to 23 bits of the row's largest element: scale sum |k| max|q| 2^-23; the scaling by d, the sum over blocks, the row's
           scale and the mask's addition: 16 u A_j + 4 u |mask_j|
+          BF16 y, many rows: k in fp16, half a step of 11 bits: 2^-11 scale sum |k| |q|
   p       2^-22 for the exponential, 2 u |s_j - max s| for its argument, and the score's
           error, doubled for the second order: rho_j
   P, V    F32 y: P as two fp16, 2^-22, and the low x low product left out, 2^-22; BF16 y: P and
@@ -37,6 +38,8 @@ def row(q, k, v, mask, scale, f32_y):
     s = kf @ q * scale
     A = (d * level) @ np.abs(q) * abs(scale)
     ds = 80 * U * A + 2.0 ** -23 * np.abs(kf).sum(1) * np.abs(q).max() * abs(scale)
+    if not f32_y:
+        ds = ds + 2.0 ** -11 * (np.abs(kf) @ np.abs(q)) * abs(scale)
     if mask is not None:
         s = s + mask
         ds = ds + 4 * U * np.abs(mask)
