@@ -33,27 +33,35 @@ typedef short fa4_v4s __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) fa4_v4s fa4_lds_v4s;
 typedef float    fa4_f4u __attribute__((ext_vector_type(4), aligned(4)));  // y at its element's alignment
 typedef uint32_t fa4_u2u __attribute__((ext_vector_type(2), aligned(2)));
-typedef uint32_t fa4_u4 __attribute__((ext_vector_type(4), aligned(4)));  // rows are 4-byte aligned
 
 constexpr float FA4_LOG2E = 1.44269504088896340736f;
 constexpr float FA4_OFF   = 8.0f;   // p = exp2(s - max + 8): fp16 parts of p keep absolute 2^-32 of the largest
-constexpr float FA4_BIG   = 8188.0f;
+constexpr float    FA4_BIG      = 8188.0f;  // past it a level times d leaves fp16
+constexpr uint32_t FA4_BIG_BITS = 0x6fffu;  // as fp16
+constexpr int      FA4_PRE_TILES = 4096;    // most tiles that a workgroup of the kernel for many rows walks
 
-// the 18 bytes of block b (d, 16 bytes of levels) as loaded: 5 words from the 4-byte
+// the 18 bytes of a block (d, 16 bytes of levels) as loaded: 5 words from the 4-byte
 // boundary at or before the block, 20 bytes that never leave the row
 struct Fa4Raw {
     uint32_t w[5];
 };
 
-__device__ __forceinline__ Fa4Raw fa4_load(const char * row, int blk) {
-    const char * p = row + ((18 * blk) & ~3);
-    const fa4_u4 x = *(const fa4_u4 *) p;
-    Fa4Raw       r;
+// The n keys of a tile from base on as a buffer: what lies past the last one (all of it for n <=
+// 0) reads as zeros without a memory access, so that every load is unconditional and a lane's
+// offset is the same in every tile (conditional loads had the compiler wait for each at once).
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t fa4_rows(const char * base, int64_t stride, int n, int row_bytes) {
+    const int bytes = n > 0 ? (n - 1) * (int) stride + row_bytes : 0;
+    return __builtin_amdgcn_make_buffer_rsrc((void *) base, (short) 0, bytes, 0x00020000);
+}
+
+__device__ __forceinline__ Fa4Raw fa4_load(__amdgpu_buffer_rsrc_t rs, int off) {
+    const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(rs, off, 0, 0);
+    Fa4Raw      r;
     r.w[0] = x.x;
     r.w[1] = x.y;
     r.w[2] = x.z;
     r.w[3] = x.w;
-    r.w[4] = *(const uint32_t *) (p + 16);
+    r.w[4] = __builtin_amdgcn_raw_buffer_load_b32(rs, off + 16, 0, 0);
     return r;
 }
 
@@ -73,6 +81,44 @@ __device__ __forceinline__ uint32_t fa4_bits(fa4_h2 v) {
 
 __device__ __forceinline__ fa4_h2 fa4_half2(uint32_t v) {
     return __builtin_bit_cast(fa4_h2, v);
+}
+
+// A lane's 8 elements of each block of a row of q: 4 from element at0 of the block on, 4 from
+// at1 on. One branch on the type around all loads.
+template <int NB, bool OS>
+__device__ __forceinline__ void fa4_q(const char * p, int type, int at0, int at1, float (*f)[8]) {
+    if (OS && type == MI_TYPE_F32) {
+        fa4_f4u v[NB][2];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            v[b][0] = *(const fa4_f4u *) (p + (b * 32 + at0) * 4);
+            v[b][1] = *(const fa4_f4u *) (p + (b * 32 + at1) * 4);
+        }
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                f[b][e] = v[b][e / 4][e % 4];
+            }
+        }
+        return;
+    }
+    fa4_u2u v[NB][2];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        v[b][0] = *(const fa4_u2u *) (p + (b * 32 + at0) * 2);
+        v[b][1] = *(const fa4_u2u *) (p + (b * 32 + at1) * 2);
+    }
+    const bool bf = !OS || type == MI_TYPE_BF16;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+            const uint32_t w = e & 2 ? v[b][e / 4].y : v[b][e / 4].x;
+            f[b][e]          = bf ? bf16_lo(w) : f16_lo(w);
+            f[b][e + 1]      = bf ? bf16_hi(w) : f16_hi(w);
+        }
+    }
 }
 
 // the B operand slots of one block of q: group g of the 4 lane groups takes bytes 4 g
@@ -97,14 +143,21 @@ __device__ __forceinline__ fa4_h8 fa4_levels(uint32_t w) {
 
 // the levels of keys (0, 2) and (1, 3) of a word (a byte per key) as fp16 numbers -8 .. 7:
 // the low nibbles, or the high ones. 0x6400 | n is 1024 + n.
+// One instruction takes both constants (the compiler, given literals, makes two).
+__device__ __forceinline__ fa4_h2 fa4_magic(uint32_t w, uint32_t mask) {
+    uint32_t r;
+    asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(r) : "v"(w), "s"(mask), "v"(0x64006400u));
+    return fa4_half2(r);
+}
+
 __device__ __forceinline__ fa4_h2 fa4_low(uint32_t w) {
     const fa4_h2 c = { (_Float16) -1032.0f, (_Float16) -1032.0f };
-    return fa4_half2((w & 0x000f000fu) | 0x64006400u) + c;
+    return fa4_magic(w, 0x000f000fu) + c;
 }
 
 __device__ __forceinline__ fa4_h2 fa4_high(uint32_t w) {
     const fa4_h2 m = { (_Float16) 0.0625f, (_Float16) 0.0625f }, c = { (_Float16) -72.0f, (_Float16) -72.0f };
-    return __builtin_elementwise_fma(fa4_half2((w & 0x00f000f0u) | 0x64006400u), m, c);
+    return __builtin_elementwise_fma(fa4_magic(w, 0x00f000f0u), m, c);
 }
 
 // Query rows (query position, head) of a KV head in tiles of 16, keys split over
@@ -180,16 +233,7 @@ __global__ void __launch_bounds__(64 * W) k_fa4_dec(const FaArgs a) {
     float qv[NB][8];
     {
         const char * qp = a.q + (int64_t) b * a.q3 + (int64_t) h * a.q2 + (int64_t) iq * a.q1;
-#pragma unroll
-        for (int blk = 0; blk < NB; ++blk) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int i = blk * 32 + 4 * q4 + (e & 3) + (e & 4) * 4;
-                qv[blk][e]  = a.tq == MI_TYPE_F32    ? load_elem<MI_TYPE_F32>(qp + (size_t) i * 4)
-                              : a.tq == MI_TYPE_BF16 ? load_elem<MI_TYPE_BF16>(qp + (size_t) i * 2)
-                                                     : load_elem<MI_TYPE_F16>(qp + (size_t) i * 2);
-            }
-        }
+        fa4_q<NB, OS>(qp, a.tq, 4 * q4, 16 + 4 * q4, qv);
     }
     float qmax = 0.0f;
 #pragma unroll
@@ -246,15 +290,23 @@ __global__ void __launch_bounds__(64 * W) k_fa4_dec(const FaArgs a) {
     const int step  = a.splits * W;
     Fa4Raw    kr[IPL], vr[IPL];
     uint16_t  mr[MS == 2 ? MT : 1][4];
-    auto      load = [&](int t) {
-        const int t0 = t * TK, last = a.n_kv - 1 - t0;
+    int       ko[IPL], vo[IPL];
+#pragma unroll
+    for (int i = 0; i < IPL; ++i) {
+        const int idx = i * 64 + lane, blk = idx % NB, key = idx / NB;
+        ko[i] = key * (int) a.k1 + ((18 * blk) & ~3);
+        vo[i] = key * (int) a.v1 + ((18 * blk) & ~3);
+    }
+    // tile t; `on` false: no tile (zeros)
+    auto load = [&](int t, bool on) {
+        const int  t0 = t * TK, last = a.n_kv - 1 - t0;
+        const int  n  = !on ? 0 : last + 1 < TK ? last + 1 : TK;
+        const auto ks = fa4_rows(kg + (int64_t) t0 * a.k1, a.k1, n, 18 * NB);
+        const auto vs = fa4_rows(vg + (int64_t) t0 * a.v1, a.v1, n, 18 * NB);
 #pragma unroll
         for (int i = 0; i < IPL; ++i) {
-            const int     idx = i * 64 + lane, blk = idx % NB;
-            const int     key = idx / NB < last ? idx / NB : last;  // past the end: the last key again
-            const int64_t at  = (int64_t) (t0 + key);
-            kr[i]             = fa4_load(kg + at * a.k1, blk);
-            vr[i]             = fa4_load(vg + at * a.v1, blk);
+            kr[i] = fa4_load(ks, ko[i]);
+            vr[i] = fa4_load(vs, vo[i]);
         }
         if constexpr (MS == 2) {
 #pragma unroll
@@ -293,7 +345,7 @@ __global__ void __launch_bounds__(64 * W) k_fa4_dec(const FaArgs a) {
             todo        = n >= F::MB ? (1u << F::MB) - 1 : (1u << n) - 1;
         }
         if (todo) {
-            load(base + (__builtin_ffs(todo) - 1) * step);
+            load(base + (__builtin_ffs(todo) - 1) * step, true);
         }
         while (todo) {
             const int i = __builtin_ffs(todo) - 1;
@@ -352,9 +404,7 @@ __global__ void __launch_bounds__(64 * W) k_fa4_dec(const FaArgs a) {
             big = __builtin_amdgcn_ballot_w64(big) != 0;
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
-            if (todo) {
-                load(base + (__builtin_ffs(todo) - 1) * step);
-            }
+            load(base + (todo ? __builtin_ffs(todo) - 1 : i) * step, todo != 0);
 
             // scores, in units of log2
             float s[MT][4], mx = -INFINITY;
@@ -600,9 +650,9 @@ __global__ void __launch_bounds__(64) k_fa4_combine(const FaArgs a) {
 //  order  a block's 32 elements lie in LDS as (half, group of 4, 0 2 1 3), the order in which
 //         masks and shifts unpack the nibbles; q is read in the same order, and the output
 //         lane's 4 values are one group of 4, put back when they are stored
-// Tiles in which a d leaves fp16's range, or a V block is not finite while some key is masked,
-// are found when they are staged and staged again (d / 16 with P or the scores * 16; v = 0
-// for keys that no row of the workgroup attends to).
+// A tile in which some d would leave fp16 is held / 16, P or its scores taken * 16; in one with a
+// block that is not finite the keys that no row of the workgroup attends to count as zeros. The
+// waves tell each other at the barrier before they lay the tile out.
 // The maximum that p refers to moves only when a row's grows by more than 2^3, so most tiles
 // need no reduction over lanes. Masks are looked up per tile in k_fa_mask_summary's bytes.
 template <int D, bool OS> struct Fa4P {
@@ -619,7 +669,6 @@ template <int D, bool OS> struct Fa4P {
     static constexpr int VB = T * VS;
     static constexpr int DB = OS ? NB * DS * 4 : 0;
     static constexpr int BUF = KB + VP * VB + DB;
-    static constexpr int CH  = 2048;                    // tiles whose mask flags are held at once
 };
 
 __device__ __forceinline__ float fa4_max_groups(float v) {  // over the 4 lane groups of 16
@@ -633,13 +682,14 @@ template <int D, bool OS, bool MSK>
 __global__ void __launch_bounds__((64 * Fa4P<D, OS>::W)) __attribute__((amdgpu_waves_per_eu(2)))
 k_fa4_pre(const FaArgs a) {
     using F          = Fa4P<D, OS>;
-    constexpr int NB = F::NB, T = F::T, RT = F::RT, W = F::W, MT = T / 16, QP = OS ? 2 : 1;
+    constexpr int NB = F::NB, T = F::T, RT = F::RT, W = F::W, QP = OS ? 2 : 1;
     constexpr int NI = 2 * T * NB;                       // blocks per tile, K's then V's
-    constexpr int IT = (NI + 64 * W - 1) / (64 * W);     // per thread
+    constexpr int IT = NI / (64 * W);                    // per thread
+    static_assert(NI % (64 * W) == 0 && T * NB % 64 == 0, "a wave's blocks are K's or V's");
     __shared__ __align__(16) char lds[2 * F::BUF];
     __shared__ uint32_t           tflag[2][W];           // 1: V's d past fp16, 2: K's, 4: V not finite
     __shared__ uint64_t           lvw[W];
-    __shared__ uint8_t            cfl[MSK ? F::CH : 1];  // 1: a live key, 2: a value that is not 0
+    __shared__ __align__(16) uint64_t wins[MSK ? FA4_PRE_TILES / 64 : 1][2];
 
     const int      tid = threadIdx.x, lane = tid & 63;
     const int      wv  = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -669,15 +719,12 @@ k_fa4_pre(const FaArgs a) {
         }
         const char * qp = a.q + (int64_t) b * a.q3 + (int64_t) h * a.q2 + (int64_t) iq * a.q1;
         float        qv[NB][8], qmax = 0.0f;
+        fa4_q<NB, OS>(qp, a.tq, 8 * q4, 8 * q4 + 4, qv);
 #pragma unroll
         for (int blk = 0; blk < NB; ++blk) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const int i = blk * 32 + 16 * (q4 >> 1) + 8 * (q4 & 1) + (e & 4) + ((e & 1) << 1 | (e >> 1 & 1));
-                qv[blk][e]  = a.tq == MI_TYPE_F32    ? load_elem<MI_TYPE_F32>(qp + (size_t) i * 4)
-                              : a.tq == MI_TYPE_BF16 ? load_elem<MI_TYPE_BF16>(qp + (size_t) i * 2)
-                                                     : load_elem<MI_TYPE_F16>(qp + (size_t) i * 2);
-                qmax        = fmaxf(qmax, fabsf(qv[blk][e]));
+                qmax = fmaxf(qmax, fabsf(qv[blk][e]));
             }
         }
         qmax           = fa4_max_groups(qmax);
@@ -689,7 +736,8 @@ k_fa4_pre(const FaArgs a) {
         for (int blk = 0; blk < NB; ++blk) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float v = qv[blk][e] * up, w = OS ? __builtin_rintf(v) : v;
+                const int   i = (e & 4) + ((e & 1) << 1 | (e >> 1 & 1));  // 0 2 1 3 of each four
+                const float v = qv[blk][i] * up, w = OS ? __builtin_rintf(v) : v;
                 qb[rt][0][blk][e] = (_Float16) w;
                 if constexpr (OS) {
                     qb[rt][1][blk][e] = (_Float16) (v - w);
@@ -710,302 +758,340 @@ k_fa4_pre(const FaArgs a) {
         }
     }
 
+    // thread: blocks i * 64 W + tid of the tile, of K (keys in order, a key's blocks together), then of V
     Fa4Raw raw[IT];
-    auto   load = [&](int t) {
-        const int t0 = t * T, last = a.n_kv - 1 - t0;
+    int    off[IT];
 #pragma unroll
-        for (int i = 0; i < IT; ++i) {
-            const int idx = i * 64 * W + tid;
-            if (NI % (64 * W) == 0 || idx < NI) {
-                const bool isv = idx >= T * NB;
-                const int  j = isv ? idx - T * NB : idx, blk = j % NB;
-                const int  key = j / NB < last ? j / NB : last;  // past the end: the last key again
-                raw[i]         = fa4_load((isv ? vg : kg) + (int64_t) (t0 + key) * (isv ? a.v1 : a.k1), blk);
-            }
-        }
+    for (int i = 0; i < IT; ++i) {
+        const bool isv = i * 64 * W + wv * 64 >= T * NB;  // uniform in the wave
+        const int  j   = i * 64 * W + tid - (isv ? T * NB : 0);
+        off[i]         = j / NB * (int) (isv ? a.v1 : a.k1) + ((18 * (j % NB)) & ~3);
+    }
+    auto load = [&](int i, int t, bool on) {  // block i of tile t; `on` false: no tile (zeros)
+        const int     t0 = t * T, n = !on ? 0 : a.n_kv - t0 < T ? a.n_kv - t0 : T;
+        const bool    isv = i * 64 * W + wv * 64 >= T * NB;
+        const int64_t st  = isv ? a.v1 : a.k1;
+        return fa4_load(fa4_rows((isv ? vg : kg) + (int64_t) t0 * st, st, n, 18 * NB), off[i]);
     };
-    // raw blocks -> buffer bf. fix: 1, 2: V's, K's d / 16; keys out of `live` as v = 0
-    auto stage = [&](int bf, uint32_t fix, uint64_t live) {
-        char *   kl = lds + bf * F::BUF, *vl = kl + F::KB;
-        float *  dl = (float *) (vl + F::VP * F::VB);
+    // flags of the blocks in raw: 1 a d of V past FA4_BIG, 2 of K, 4 one that is not finite
+    auto flags = [&]() -> uint32_t {
         uint32_t fl = 0;
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
-            const int idx = i * 64 * W + tid;
-            if (NI % (64 * W) == 0 || idx < NI) {
-                const bool isv = idx >= T * NB;
-                const int  j = isv ? idx - T * NB : idx, blk = j % NB, key = j / NB;
-                float      d;
-                uint32_t   w[4];
-                fa4_block(raw[i], blk, d, w);
-                if (isv) {
-                    d = live >> key & 1 ? d : 0.0f;
-                    fl |= fabsf(d) <= FA4_BIG ? 0u : fabsf(d) <= 65504.0f ? 1u : 4u;
-                    d = fix & 1 ? d * 0.0625f : d;
-                } else if (!OS) {
-                    fl |= fabsf(d) > FA4_BIG && fabsf(d) <= 65504.0f ? 2u : 0u;
-                    d = fix & 2 ? d * 0.0625f : d;
-                } else {
-                    dl[blk * F::DS + key] = d;
-                }
-                const _Float16 dh = (_Float16) d;
-                const fa4_h2   dd = { dh, dh };
-                uint32_t       q[16], ql[16];
+            const bool     isv = i * 64 * W + wv * 64 >= T * NB;
+            const int      j   = i * 64 * W + tid - (isv ? T * NB : 0), blk = j % NB;
+            const uint32_t mag = (blk & 1 ? raw[i].w[0] >> 16 : raw[i].w[0]) & 0x7fffu;
+            if (__builtin_amdgcn_ballot_w64(mag > FA4_BIG_BITS) != 0) {
+                fl |= (isv ? 1u : 2u) | (__builtin_amdgcn_ballot_w64(mag >= 0x7c00u) != 0 ? 4u : 0u);
+            }
+        }
+        return fl;
+    };
+    // block i of a tile with the flags fl -> buffer bf: V's, K's d / 16 with flag 1, 2; zeros for keys
+    // that are not in `live` with flag 4
+    auto stage = [&](int i, const Fa4Raw & rw, int bf, uint32_t fl, uint64_t live) {
+        char *     kl = lds + bf * F::BUF, *vl = kl + F::KB;
+        float *    dl  = (float *) (vl + F::VP * F::VB);
+        const bool isv = i * 64 * W + wv * 64 >= T * NB;
+        const int  j   = i * 64 * W + tid - (isv ? T * NB : 0), blk = j % NB, key = j / NB;
+        float      d;
+        uint32_t   w[4];
+        fa4_block(rw, blk, d, w);
+        if (fl & 4) {
+            d = live >> key & 1 ? d : 0.0f;
+        }
+        if (OS && !isv) {
+            dl[blk * F::DS + key] = d;  // fp32: nothing to scale
+        }
+        d *= fl & (isv ? 1u : 2u) ? 0.0625f : 1.0f;
+        const _Float16 dh = (_Float16) d;
+        const fa4_h2 dd = { dh, dh };
+        uint32_t     q[16], ql[16];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < 4; ++e) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {  // low (0 2), low (1 3), high (0 2), high (1 3)
-                        const uint32_t x = k & 1 ? w[e] >> 8 : w[e];
-                        const fa4_h2   n = k & 2 ? fa4_high(x) : fa4_low(x), v = n * dd;
-                        const int      at = (k & 2) * 4 + 2 * e + (k & 1);
-                        q[at] = OS && !isv ? fa4_bits(n) : fa4_bits(v);
-                        if constexpr (OS) {
-                            ql[at] = fa4_bits(__builtin_elementwise_fma(n, dd, -v));
-                        }
-                    }
-                }
-                char * p = isv ? vl + key * F::VS + blk * 64 : kl + key * F::KS + blk * 64;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    *(uint4 *) (p + 16 * e) = make_uint4(q[4 * e], q[4 * e + 1], q[4 * e + 2], q[4 * e + 3]);
-                    if constexpr (OS) {
-                        if (isv) {
-                            *(uint4 *) (p + F::VB + 16 * e) = make_uint4(ql[4 * e], ql[4 * e + 1], ql[4 * e + 2], ql[4 * e + 3]);
-                        }
-                    }
+            for (int k = 0; k < 4; ++k) {  // low (0 2), low (1 3), high (0 2), high (1 3)
+                const uint32_t x  = k & 1 ? w[e] >> 8 : w[e];
+                const fa4_h2   n  = k & 2 ? fa4_high(x) : fa4_low(x), v = n * dd;
+                const int      at = (k & 2) * 4 + 2 * e + (k & 1);
+                q[at] = OS && !isv ? fa4_bits(n) : fa4_bits(v);
+                if constexpr (OS) {
+                    ql[at] = fa4_bits(__builtin_elementwise_fma(n, dd, -v));
                 }
             }
         }
-        fl = (__builtin_amdgcn_ballot_w64(fl & 1) ? 1u : 0u) | (__builtin_amdgcn_ballot_w64(fl & 2) ? 2u : 0u) |
-             (__builtin_amdgcn_ballot_w64(fl & 4) ? 4u : 0u);
-        if (lane == 0) {
-            tflag[bf][wv] = fl;
+        char * p = isv ? vl + key * F::VS + blk * 64 : kl + key * F::KS + blk * 64;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            *(uint4 *) (p + 16 * e) = make_uint4(q[4 * e], q[4 * e + 1], q[4 * e + 2], q[4 * e + 3]);
+            if constexpr (OS) {
+                if (isv) {
+                    *(uint4 *) (p + F::VB + 16 * e) = make_uint4(ql[4 * e], ql[4 * e + 1], ql[4 * e + 2], ql[4 * e + 3]);
+                }
+            }
         }
     };
 
     const int ntile = (a.n_kv + T - 1) / T;
     const int tbeg  = (int) ((int64_t) ntile * split / a.splits), tend = (int) ((int64_t) ntile * (split + 1) / a.splits);
     const int iq0 = r0 / a.rk, iq1 = (r0 + F::BQ < a.rows ? r0 + F::BQ - 1 : a.rows - 1) / a.rk;
-    for (int cb = tbeg; cb < tend; cb += F::CH) {
-        const int ce = tend - cb < F::CH ? tend : cb + F::CH;
-        if constexpr (MSK) {
-            const int nts = (a.n_kv + 63) / 64, nh = a.rk < a.mne2 ? a.rk : a.mne2;
-            __syncthreads();  // the chunk before is done with its flags
-            for (int t = cb + tid; t < ce; t += 64 * W) {
-                uint32_t f = 0;
-                for (int hh = 0; hh < nh; ++hh) {
-                    const int       mh = (int) (b % (uint32_t) a.mne3) * a.mne2 + ((int) g * a.rk + hh) % a.mne2;
-                    const uint8_t * mp = a.msum + ((int64_t) mh * a.ngq) * nts + t * T / 64;
-                    for (int gr = iq0 >> 4; gr <= iq1 >> 4; ++gr) {
-                        f |= mp[(int64_t) gr * nts];
-                    }
+    // the tiles with a live key, and those with values that are not 0 (`dirty`), a bit per tile: a wave
+    // reads the summary bytes of the workgroup's rows for 64 tiles at a time
+    if constexpr (MSK) {
+        const int nts = (a.n_kv + 63) / 64, nh = a.rk < a.mne2 ? a.rk : a.mne2;
+        for (int w0 = tbeg + wv * 64; w0 < tend; w0 += 64 * W) {
+            const int t = w0 + lane < tend ? w0 + lane : tend - 1;
+            uint32_t  f = 0;
+            for (int hh = 0; hh < nh; ++hh) {
+                const int       mh = (int) (b % (uint32_t) a.mne3) * a.mne2 + ((int) g * a.rk + hh) % a.mne2;
+                const uint8_t * mp = a.msum + ((int64_t) mh * a.ngq) * nts + t * T / 64;
+#pragma unroll 4
+                for (int gr = iq0 >> 4; gr <= iq1 >> 4; ++gr) {
+                    f |= mp[(int64_t) gr * nts];
                 }
-                cfl[t - cb] = (uint8_t) f;
             }
-            __syncthreads();
-        }
-        auto next = [&](int t) {  // the first tile from t on with a live key, or ce
-            if constexpr (MSK) {
-                while (t < ce) {
-                    const uint64_t v = __builtin_amdgcn_ballot_w64(t + lane < ce && (cfl[t + lane - cb < F::CH ? t + lane - cb : 0] & 1));
-                    if (v) {
-                        return t + (int) __builtin_ctzll(v);
-                    }
-                    t += 64;
-                }
-                return ce;
-            } else {
-                return t;
+            const uint64_t x = __builtin_amdgcn_ballot_w64(w0 + lane < tend && (f & 1));
+            const uint64_t y = __builtin_amdgcn_ballot_w64((f & 2) != 0);
+            if (lane == 0) {
+                wins[(w0 - tbeg) / 64][0] = x;
+                wins[(w0 - tbeg) / 64][1] = y;
             }
-        };
-        int t = next(cb);
-        if (t >= ce) {
-            continue;
-        }
-        load(t);
-        int bf = 0;
-        stage(0, 0, ~0ull);
-        int tn = next(t + 1);
-        if (tn < ce) {
-            load(tn);
         }
         __syncthreads();
+    }
+    int      wb = tbeg - 64;
+    uint64_t lv = 0, nz = 0;
+    auto     next = [&](bool & dirty) -> int {  // the next tile to walk, tend after the last
+        if constexpr (MSK) {
+            while (lv == 0) {
+                wb += 64;
+                if (wb >= tend) {
+                    wb = tend;  // asked again: still none
+                    return tend;
+                }
+                const uint4 x = *(const uint4 *) wins[(wb - tbeg) / 64];
+                lv = (uint64_t) (uint32_t) __builtin_amdgcn_readfirstlane((int) x.y) << 32 |
+                     (uint32_t) __builtin_amdgcn_readfirstlane((int) x.x);
+                nz = (uint64_t) (uint32_t) __builtin_amdgcn_readfirstlane((int) x.w) << 32 |
+                     (uint32_t) __builtin_amdgcn_readfirstlane((int) x.z);
+            }
+            const int i = (int) __builtin_ctzll(lv);
+            lv &= lv - 1;
+            dirty = nz >> i & 1;
+            return wb + i;
+        } else {
+            dirty = false;
+            wb    = wb < tbeg ? tbeg : wb + 1;
+            return wb < tend ? wb : tend;
+        }
+    };
+    // the flags that every wave found for a tile; the keys that some row of the workgroup attends to
+    // where one is not finite
+    auto agree = [&](int bf, int t, uint64_t & live) -> uint32_t {
+        uint32_t fl = 0;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            fl |= tflag[bf][w];
+        }
+        fl = __builtin_amdgcn_readfirstlane(fl);
+        if (fl & 4) {
+            live = 0;
+#pragma unroll 1
+            for (int k = 0; k < T; k += 4) {
+                const int key = t * T + k + q4;
+                bool      on  = false;
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    bool x = key < a.n_kv;
+                    if constexpr (MSK) {
+                        x = x && *(const uint16_t *) (mrow[rt] + (int64_t) (x ? key : 0) * 2) != 0xFC00u;
+                    }
+                    on = on || x;
+                }
+                const uint64_t v = __builtin_amdgcn_ballot_w64(on);
+#pragma unroll 1
+                for (int gr = 0; gr < 4; ++gr) {
+                    live |= (uint64_t) ((v >> (16 * gr) & 0xffffu) != 0) << (k + gr);
+                }
+            }
+            if (lane == 0) {
+                lvw[wv] = live;
+            }
+            __syncthreads();
+            for (int w = 0; w < W; ++w) {
+                live |= lvw[w];
+            }
+            __syncthreads();  // lvw may be written again
+        }
+        return fl;
+    };
+    bool dirty, dirty_n, dirty_2;
+    int  t = next(dirty), bf = 0;
+    if (t < tend) {
+#pragma unroll
+        for (int i = 0; i < IT; ++i) {
+            raw[i] = load(i, t, true);
+        }
+        tflag[0][wv] = flags();
+        __syncthreads();
+        uint64_t live = 0;
+        uint32_t fl   = agree(0, t, live);
+        int      tn   = next(dirty_n);
+#pragma unroll
+        for (int i = 0; i < IT; ++i) {
+            stage(i, raw[i], 0, fl, live);
+            raw[i] = load(i, tn, tn < tend);
+        }
+        tflag[1][wv] = flags();
+        __syncthreads();
         while (true) {
-            if (tn < ce) {
-                stage(bf ^ 1, 0, ~0ull);
-            }
-            const int t2 = tn < ce ? next(tn + 1) : ce;
-            if (t2 < ce) {
-                load(t2);
-            }
+            const int      t2 = next(dirty_2);
+            const uint32_t fn = agree(bf ^ 1, tn, live);  // the next tile's
             const int    t0 = t * T;
             const char * kl = lds + bf * F::BUF;
             const char * vl = kl + F::KB;
             const float * dl = (const float *) (vl + F::VP * F::VB);
-            const bool   clean = t0 + T <= a.n_kv && (!MSK || !(cfl[MSK ? t - cb : 0] & 2));
-            uint32_t     fl    = 0;
+            const bool   clean = t0 + T <= a.n_kv && !dirty;
+            const float  kf = !OS && (fl & 2) ? 16.0f : 1.0f;  // what the scores are to be multiplied by
+            if constexpr (OS) {  // fewer registers are left for what the product's instructions could hide
 #pragma unroll
-            for (int w = 0; w < W; ++w) {
-                fl |= tflag[bf][w];
-            }
-            fl = __builtin_amdgcn_readfirstlane(fl);
-            float kf = 1.0f;  // what the scores are to be multiplied by
-            if (fl != 0) {
-                // some d past fp16, or a V block that is not finite: the tile again, scaled, without
-                // the keys that no row attends to
-                uint64_t live = 0;
-                if (!clean && (fl & 4)) {
-                    for (int rt = 0; rt < RT; ++rt) {
-                        for (int k = 0; k < T; k += 4) {
-                            const int  key = k + q4;
-                            bool       on = t0 + key < a.n_kv;
-                            if constexpr (MSK) {
-                                on = on && *(const uint16_t *) (mrow[rt] + (int64_t) (on ? t0 + key : 0) * 2) != 0xFC00u;
-                            }
-                            const uint64_t v = __builtin_amdgcn_ballot_w64(on);
-                            for (int gr = 0; gr < 4; ++gr) {
-                                live |= (uint64_t) ((v >> (16 * gr) & 0xffffu) != 0) << (k + gr);
-                            }
-                        }
-                    }
-                    if (lane == 0) {
-                        lvw[wv] = live;
-                    }
-                    __syncthreads();
-                    for (int w = 0; w < W; ++w) {
-                        live |= lvw[w];
-                    }
-                } else {
-                    live = ~0ull;
+                for (int i = 0; i < IT; ++i) {
+                    stage(i, raw[i], bf ^ 1, fn, live);
+                    raw[i] = load(i, t2, t2 < tend);
                 }
-                __syncthreads();  // every wave has read the tile's flags
-                load(t);
-                stage(bf, fl & 3, live);
-                if (t2 < ce) {
-                    load(t2);
-                }
-                __syncthreads();
-                kf = fl & 2 ? 16.0f : 1.0f;
             }
-
-            fa4_f4 s[RT][MT];
+            const float pinv = fl & 1 ? 0.0625f : 1.0f;  // P is held 16 times as large where V is held / 16
+            const float poff = fl & 1 ? FA4_OFF + 4.0f : FA4_OFF;
+            // 32 keys at a time: few enough scores and operands that the LDS reads of both products can be
+            // in flight before the first is used
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-                const char * kp = kl + (16 * mt + c16) * F::KS + q4 * 16;
+            for (int kk = 0; kk < T / 32; ++kk) {
+                fa4_h8 kx[2][NB];
+#pragma unroll
+                for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+                    for (int blk = 0; blk < NB; ++blk) {
+                        kx[mt][blk] = *(const fa4_h8 *) (kl + (32 * kk + 16 * mt + c16) * F::KS + q4 * 16 + blk * 64);
+                    }
+                }
+                // mask values of the lane's scores in units of log2, 4 keys a load where rows are 8-byte aligned
+                fa4_f4 mk[RT][2];
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) {
-                    s[rt][mt] = fa4_f4{ 0.0f, 0.0f, 0.0f, 0.0f };
+                    mk[rt][0] = mk[rt][1] = fa4_f4{ 0.0f, 0.0f, 0.0f, 0.0f };
                 }
+                if (!clean) {
 #pragma unroll
-                for (int blk = 0; blk < NB; ++blk) {
-                    const fa4_h8 x = *(const fa4_h8 *) (kp + blk * 64);
-                    if constexpr (OS) {
-                        const fa4_f4 dk = *(const fa4_f4 *) (dl + blk * F::DS + 16 * mt + 4 * q4);
+                    for (int rt = 0; rt < RT; ++rt) {
+                        uint32_t x[2][2] = {};
+                        if constexpr (MSK) {
+                            const char * mp = mrow[rt] + (int64_t) (t0 + 32 * kk + 4 * q4) * 2;
+                            if (a.mvec && t0 + T <= a.n_kv) {
+                                const uint2 y = *(const uint2 *) mp, z = *(const uint2 *) (mp + 32);
+                                x[0][0] = y.x;
+                                x[0][1] = y.y;
+                                x[1][0] = z.x;
+                                x[1][1] = z.y;
+                            } else {
 #pragma unroll
-                        for (int rt = 0; rt < RT; ++rt) {
-#pragma unroll
-                            for (int p = 1; p >= 0; --p) {
-                                const fa4_f4 acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                                    x, qb[rt][OS ? p : 0][blk], fa4_f4{ 0.0f, 0.0f, 0.0f, 0.0f }, 0, 0, 0);
-#pragma unroll
-                                for (int r = 0; r < 4; ++r) {
-                                    s[rt][mt][r] = __builtin_fmaf(acc[r], dk[r], s[rt][mt][r]);
+                                for (int e = 0; e < 8; ++e) {
+                                    const int      key = t0 + 32 * kk + 16 * (e / 4) + 4 * q4 + e % 4;
+                                    const int      at  = key < a.n_kv ? key : a.n_kv - 1;
+                                    const uint32_t y   = *(const uint16_t *) (mrow[rt] + (int64_t) at * 2);
+                                    x[e / 4][e % 4 / 2] |= y << (16 * (e % 2));
                                 }
                             }
                         }
-                    } else {
 #pragma unroll
-                        for (int rt = 0; rt < RT; ++rt) {
-                            s[rt][mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, qb[rt][0][blk], s[rt][mt], 0, 0, 0);
+                        for (int e = 0; e < 8; ++e) {
+                            const bool  in = t0 + 32 * kk + 16 * (e / 4) + 4 * q4 + e % 4 < a.n_kv;
+                            const float y  = (e & 1 ? f16_hi(x[e / 4][e % 4 / 2]) : f16_lo(x[e / 4][e % 4 / 2])) * FA4_LOG2E;
+                            mk[rt][e / 4][e % 4] = in ? y : -INFINITY;
                         }
                     }
                 }
-            }
-            float fac[RT], lm[RT];
+                fa4_f4 s[RT][2];
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                fac[rt] = qs[rt] * kf;
-            }
-            if (!clean) {  // scores with their mask values, in units of log2
+                for (int mt = 0; mt < 2; ++mt) {
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
+                    for (int rt = 0; rt < RT; ++rt) {
+                        s[rt][mt] = fa4_f4{ 0.0f, 0.0f, 0.0f, 0.0f };
+                    }
 #pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) {
+                    for (int blk = 0; blk < NB; ++blk) {
+                        if constexpr (OS) {
+                            const fa4_f4 dk = *(const fa4_f4 *) (dl + blk * F::DS + 32 * kk + 16 * mt + 4 * q4);
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const int  key = t0 + 16 * mt + 4 * q4 + r;
-                            const bool in  = key < a.n_kv;
-                            float      mk  = in ? 0.0f : -INFINITY;
-                            if constexpr (MSK) {
-                                const float x = f16_lo(*(const uint16_t *) (mrow[rt] + (int64_t) (in ? key : a.n_kv - 1) * 2));
-                                mk            = in ? x * FA4_LOG2E : -INFINITY;
+                            for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+                                for (int p = 1; p >= 0; --p) {
+                                    const fa4_f4 acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                                        kx[mt][blk], qb[rt][OS ? p : 0][blk], fa4_f4{ 0.0f, 0.0f, 0.0f, 0.0f }, 0, 0, 0);
+#pragma unroll
+                                    for (int r = 0; r < 4; ++r) {
+                                        s[rt][mt][r] = __builtin_fmaf(acc[r], dk[r], s[rt][mt][r]);
+                                    }
+                                }
                             }
-                            s[rt][mt][r] = mk == -INFINITY ? -INFINITY : __builtin_fmaf(s[rt][mt][r], fac[rt], mk);
+                        } else {
+#pragma unroll
+                            for (int rt = 0; rt < RT; ++rt) {
+                                s[rt][mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kx[mt][blk], qb[rt][0][blk], s[rt][mt], 0, 0, 0);
+                            }
                         }
                     }
-                    fac[rt] = 1.0f;
                 }
-            }
-            bool grow = false;
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                float x = -INFINITY;
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-                    x = fmaxf(fmaxf(x, s[rt][mt][0]), s[rt][mt][1]);
-                    x = fmaxf(fmaxf(x, s[rt][mt][2]), s[rt][mt][3]);
+                // the next tile's blocks, while the product runs
+                if (!OS && kk < IT) {
+                    stage(kk, raw[kk], bf ^ 1, fn, live);  // past the last tile: zeros
+                    raw[kk] = load(kk, t2, t2 < tend);
                 }
-                lm[rt] = x * fac[rt];
-                grow   = grow || lm[rt] > m[rt] + 3.0f;
-            }
-            if (__builtin_amdgcn_ballot_w64(grow) != 0) {
+                float lm[RT];
+                bool  grow = false;
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) {
-                    const float mn = fmaxf(m[rt], fa4_max_groups(lm[rt]));
-                    const float al = m[rt] == mn ? 1.0f : __builtin_amdgcn_exp2f(m[rt] - mn);
-                    m[rt]          = mn;
-                    l[rt] *= al;
-#pragma unroll
-                    for (int i = 0; i < 2 * NB; ++i) {
-                        o[rt][i] *= al;
-                    }
-                }
-            }
-            const float pf = fl & 1 ? 16.0f : 1.0f;
-            fa4_h8      ph[RT][T / 32], pl[OS ? RT : 1][T / 32];
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                const float mu = FA4_OFF - (m[rt] == -INFINITY ? 0.0f : m[rt]);
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rt][mt][r], fac[rt], mu));
-                        l[rt] += p;
-                        s[rt][mt][r] = p;
-                    }
-                }
-                if (fl & 1) {
-#pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) {
-                        s[rt][mt] *= pf;
-                    }
-                }
-#pragma unroll
-                for (int kk = 0; kk < T / 32; ++kk) {
+                    const float fac = qs[rt] * kf;
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        const float    p = s[rt][2 * kk + e / 4][e & 3];
-                        const _Float16 h = (_Float16) p;
-                        ph[rt][kk][e]    = h;
-                        if constexpr (OS) {
-                            pl[rt][kk][e] = (_Float16) (p - (float) h);
+                        s[rt][e / 4][e % 4] = __builtin_fmaf(s[rt][e / 4][e % 4], fac, mk[rt][e / 4][e % 4]);
+                    }
+                    float x = fmaxf(fmaxf(s[rt][0][0], s[rt][0][1]), s[rt][0][2]);
+                    x       = fmaxf(fmaxf(x, s[rt][0][3]), s[rt][1][0]);
+                    x       = fmaxf(fmaxf(x, s[rt][1][1]), s[rt][1][2]);
+                    lm[rt]  = fmaxf(x, s[rt][1][3]);
+                    grow    = grow || lm[rt] > m[rt] + 3.0f;
+                }
+                if (__builtin_amdgcn_ballot_w64(grow) != 0) {
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) {
+                        const float mn = fmaxf(m[rt], fa4_max_groups(lm[rt]));
+                        const float al = m[rt] == mn ? 1.0f : __builtin_amdgcn_exp2f(m[rt] - mn);
+                        m[rt]          = mn;
+                        l[rt] *= al;
+#pragma unroll
+                        for (int i = 0; i < 2 * NB; ++i) {
+                            o[rt][i] *= al;
                         }
                     }
                 }
-            }
+                fa4_h8 ph[RT], pl[RT];
 #pragma unroll
-            for (int kk = 0; kk < T / 32; ++kk) {
+                for (int rt = 0; rt < RT; ++rt) {
+                    const float mu = poff - (m[rt] == -INFINITY ? 0.0f : m[rt]);
+                    float       p[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        p[e] = __builtin_amdgcn_exp2f(s[rt][e / 4][e % 4] + mu);
+                    }
+                    l[rt] = __builtin_fmaf(((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7])), pinv, l[rt]);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        ph[rt][e] = (_Float16) p[e];
+                        if constexpr (OS) {
+                            pl[rt][e] = (_Float16) (p[e] - (float) ph[rt][e]);
+                        }
+                    }
+                }
                 // lane m of a group of 16 addresses key m / 4 of the group's 4, positions 4 (m % 4)
                 const char * vp = vl + (32 * kk + 4 * q4 + (c16 >> 2)) * F::VS + (c16 & 3) * 8;
 #pragma unroll
@@ -1020,23 +1106,26 @@ k_fa4_pre(const FaArgs a) {
 #pragma unroll
                     for (int rt = 0; rt < RT; ++rt) {
                         fa4_f4 & oo = o[rt][dt];
-                        oo          = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[0], ph[rt][kk], oo, 0, 0, 0);
+                        oo          = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[0], ph[rt], oo, 0, 0, 0);
                         if constexpr (OS) {
-                            oo = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[0], pl[rt][kk], oo, 0, 0, 0);
-                            oo = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[F::VP - 1], ph[rt][kk], oo, 0, 0, 0);
+                            oo = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[0], pl[rt], oo, 0, 0, 0);
+                            oo = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[F::VP - 1], ph[rt], oo, 0, 0, 0);
                         }
                     }
                 }
             }
-            if (tn >= ce) {
+            if (tn >= tend) {
                 break;
             }
+            tflag[bf][wv] = flags();
             __syncthreads();
-            t  = tn;
-            tn = t2;
+            fl      = fn;
+            t       = tn;
+            tn      = t2;
+            dirty   = dirty_n;
+            dirty_n = dirty_2;
             bf ^= 1;
         }
-        __syncthreads();  // the next chunk stages into the buffers
     }
 
 #pragma unroll
@@ -1102,25 +1191,27 @@ void flash_attn_q4_plan(FaArgs & a, int D) {
     if (a.nb == 0 || a.rows == 0 || tiles == 0) {
         return;
     }
-    if (a.n_kv > 1 << 27) {
-        a.splits = 0;  // a wave's walk counts keys in 32 bits, 8 tiles of every wave ahead
+    if (a.n_kv > 1 << 27 || a.k1 >= 1 << 25 || a.v1 >= 1 << 25) {
+        a.splits = 0;  // keys are counted in 32 bits, 8 tiles of every wave ahead; a tile's offsets too
         return;
     }
     a.mfma = a.rows > FA4_DEC_ROWS && a.ngq <= 65535 && (int64_t) a.nb * a.nh <= 65535;
-    int64_t items, want, most;
+    int64_t items, want, most, least = 1;
     if (a.mfma) {
         // the workspace is sized without y: its type (rows per workgroup) must not change the splits
         a.rblocks = (a.rows + 127) / 128;
         items     = (int64_t) a.nb * a.nkv * a.rblocks;
         want      = (int64_t) num_cus() * 2 / items;
         most      = (tiles + 7) / 8;
+        least     = (tiles + FA4_PRE_TILES - 1) / FA4_PRE_TILES;
     } else {
         items = (int64_t) a.nb * a.nkv * a.rblocks;
         // enough waves for 16 per CU, at most one tile each
         want = ((int64_t) num_cus() * 16 / FA4_W + items - 1) / items;
         most = (tiles + FA4_W - 1) / FA4_W;
     }
-    a.splits = (int) (want < 1 ? 1 : want < most ? want : most);
+    want     = want < most ? want : most;
+    a.splits = (int) (want < least ? least : want);
     if (items * a.splits >= ((int64_t) 1 << 31)) {
         a.splits = 0;  // more workgroups than a grid has
     }
