@@ -40,3 +40,32 @@ def test_refused(t):
 def test_dtype_refused():
     with pytest.raises(TypeError):
         ops.desc(DTensor(Mem(), (4,), "u8"))
+
+
+def test_a_call_s_argument_follows_the_view():
+    """The argument kept with a view is made anew when the view, its buffer's address or its block type changes."""
+    class Moving:
+        ptr, nbytes = 1 << 20, 4096
+
+    def data(t):
+        a = ops._p(t)._obj
+        return a.data, a.type, list(a.ne), list(a.nb)
+
+    x = DTensor(Moving(), (4, 68), "u8")
+    q = ops.Q8(x)
+    first = ops._p(q)
+    assert ops._p(q) is first and ops._p(ops.Q8(x)) is first
+    assert data(q) == (1 << 20, Q8_0, [64, 4, 1, 1], [34, 68, 272, 272])
+    y = DTensor(Moving(), (4, 36), "u8")
+    assert data(ops.Q4(y))[1] == 2
+    y.shape = (2, 36)
+    assert data(ops.Q4(y))[2] == [64, 2, 1, 1]
+    y.offset = 72
+    assert data(ops.Q4(y))[0] == (1 << 20) + 72
+    y.buf.ptr = 1 << 21
+    assert data(ops.Q4(y))[0] == (1 << 21) + 72
+    z = DTensor(Moving(), (8,), "f32")
+    assert data(z)[1] == F32
+    z.dtype = "i32"
+    assert data(z)[1] == 26
+    assert ops._p(None) is None
