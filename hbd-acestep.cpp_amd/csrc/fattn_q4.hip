@@ -11,11 +11,9 @@
 //         of the row's largest; the matrix cores' sums of whole numbers are exact, where
 //         sums of 24-bit terms are cut at each step (measured over the LM's decode size:
 //         y off by 4.1e-6 with two fp16 of any size, 2-norm over 2-norm, torch's fp32 6e-7).
-//  levels as fp16 operands are the nibbles themselves: 0x000n is n 2^-24 and 0x00n0
-//         16 n 2^-24, subnormals that the matrix cores take as they are, so two
-//         ANDs and a shift per pair make an operand; q's elements that meet a high
-//         nibble are divided by 16, 2^24 goes into the row's scale, and the -8 into
-//         the accumulator's start, -8 sum(q) of the block.
+//  levels as fp16 numbers -8 .. 7, by one mask-and-or and one packed add each two (the
+//         nibbles' bits as they are, subnormals n 2^-24, with the -8 in the accumulator's
+//         start, took fewer instructions but 4 registers a block for that start).
 //  P, V   F32 y: P and v = (level - 8) d as a high and a low fp16 each (v exact, P to
 //         22 bits), three products; BF16 y: one fp16 each (2^-11 against y's 2^-8).
 //         d above 8188 would leave fp16: tiles with one scale v by 2^-4, P by 2^4.
@@ -121,28 +119,8 @@ __device__ __forceinline__ void fa4_q(const char * p, int type, int at0, int at1
     }
 }
 
-// the B operand slots of one block of q: group g of the 4 lane groups takes bytes 4 g
-// .. 4 g + 3 of the levels; v: elements 4 g + (0..3), then 16 + 4 g + (0..3)
-__device__ __forceinline__ void fa4_slots(const float * v, float * s) {
-    s[0] = v[0];
-    s[1] = v[2];
-    s[2] = v[4] * 0.0625f;
-    s[3] = v[6] * 0.0625f;
-    s[4] = v[1];
-    s[5] = v[3];
-    s[6] = v[5] * 0.0625f;
-    s[7] = v[7] * 0.0625f;
-}
-
-// 8 levels of a word of 4 bytes as an A operand, in the slots' order
-__device__ __forceinline__ fa4_h8 fa4_levels(uint32_t w) {
-    const uint32_t v = w >> 8;
-    const u32x4    r = { w & 0x000f000fu, w & 0x00f000f0u, v & 0x000f000fu, v & 0x00f000f0u };
-    return __builtin_bit_cast(fa4_h8, r);
-}
-
-// the levels of keys (0, 2) and (1, 3) of a word (a byte per key) as fp16 numbers -8 .. 7:
-// the low nibbles, or the high ones. 0x6400 | n is 1024 + n.
+// Bytes 0 and 2 of a word as two fp16 numbers -8 .. 7: the low nibbles, or the high ones
+// (bytes 1 and 3 of it: of w >> 8). 0x6400 | n is 1024 + n.
 // One instruction takes both constants (the compiler, given literals, makes two).
 __device__ __forceinline__ fa4_h2 fa4_magic(uint32_t w, uint32_t mask) {
     uint32_t r;
@@ -160,6 +138,20 @@ __device__ __forceinline__ fa4_h2 fa4_high(uint32_t w) {
     return __builtin_elementwise_fma(fa4_magic(w, 0x00f000f0u), m, c);
 }
 
+// 8 levels of a word of 4 bytes as an A operand: bytes 0 2 low, 0 2 high, 1 3 low, 1 3 high.
+// Group g of the 4 lane groups takes bytes 4 g .. 4 g + 3 of a block's levels, so the slots
+// are elements 4 g + { 0, 2, 16, 18, 1, 3, 17, 19 }.
+__device__ __forceinline__ fa4_h8 fa4_levels(uint32_t w) {
+    const uint32_t v = w >> 8;
+    const u32x4    r = { fa4_bits(fa4_low(w)), fa4_bits(fa4_high(w)), fa4_bits(fa4_low(v)), fa4_bits(fa4_high(v)) };
+    return __builtin_bit_cast(fa4_h8, r);
+}
+
+// slot e of them as an index into the 4 elements from 4 g on, then the 4 from 16 + 4 g on
+__device__ __forceinline__ constexpr int fa4_slot(int e) {
+    return (e & 2) * 2 + (e & 1) * 2 + (e >> 2);
+}
+
 // Query rows (query position, head) of a KV head in tiles of 16, keys split over
 // workgroups of W waves, a wave taking every (splits * W)-th tile of TK keys. With
 // v_mfma_f32_16x16x32_f16 (lane l: A[l%16][8(l/16)+e], B[8(l/16)+e][l%16],
@@ -175,7 +167,7 @@ __device__ __forceinline__ fa4_h2 fa4_high(uint32_t w) {
 // a key that no row attends to counts as v = 0 whatever its bytes are.
 template <int D> struct Fa4 {
     static constexpr int NB   = D / 32;
-    static constexpr int TK   = D == 256 ? 32 : 64;  // keys per tile
+    static constexpr int TK   = D == 64 ? 64 : 32;  // keys per tile
     static constexpr int IPL  = TK * NB / 64;        // blocks per lane and tile, of K and of V
     static constexpr int MT   = TK / 16;
     static constexpr int KROW = 16 * NB;             // bytes of levels per key
@@ -187,7 +179,7 @@ template <int D> struct Fa4 {
     static constexpr int DVB  = NB * DS * 2;
     static constexpr int MB   = 8;                   // tiles whose mask is read at once
     static constexpr int WAVE = KB + VB + DKB + DVB; // LDS bytes per wave, without the mask
-    static constexpr int DC   = D < 128 ? D : 128;   // columns merged at a time
+    static constexpr int DC   = 64;                  // columns merged at a time
     static __device__ __forceinline__ int koff(int key) { return key * KROW + key / RPP * 4 * NB; }
     static __device__ __forceinline__ int voff(int key) { return key * KROW + key / RPP * 16; }
 };
@@ -250,32 +242,15 @@ __global__ void __launch_bounds__(64 * W) k_fa4_dec(const FaArgs a) {
     const float up = __uint_as_float((uint32_t) (127 + 10 - ex) << 23);
     const float qs = a.scale * FA4_LOG2E * __uint_as_float((uint32_t) (127 - 10 + ex) << 23);
     fa4_h8      qb[QP][NB];
-    float       c0[QP][NB];
 #pragma unroll
     for (int blk = 0; blk < NB; ++blk) {
-        float s[8], sum[QP] = {};
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            qv[blk][e] *= up;
-        }
-        float part[8], rest[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            part[e] = QP == 2 ? __builtin_rintf(qv[blk][e]) : qv[blk][e];
-            rest[e] = qv[blk][e] - part[e];
-        }
-#pragma unroll
-        for (int p = 0; p < QP; ++p) {
-            fa4_slots(p ? rest : part, s);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                qb[p][blk][e] = (_Float16) s[e];
-                // slots 2, 3, 6, 7 meet 16 times the level
-                sum[p] += (float) qb[p][blk][e] * (e & 2 ? 16.0f : 1.0f);
+            const float v = qv[blk][fa4_slot(e)] * up, w = OS ? __builtin_rintf(v) : v;
+            qb[0][blk][e] = (_Float16) w;
+            if constexpr (OS) {
+                qb[1][blk][e] = (_Float16) (v - w);
             }
-            sum[p] += __shfl_xor(sum[p], 16, 64);
-            sum[p] += __shfl_xor(sum[p], 32, 64);
-            c0[p][blk] = sum[p] * (-8.0f / 16777216.0f);
         }
     }
 
@@ -392,7 +367,7 @@ __global__ void __launch_bounds__(64 * W) k_fa4_dec(const FaArgs a) {
                 for (int e = 0; e < 4; ++e) {
                     *(uint32_t *) (kp + e * 4 * NB) = q[e];
                 }
-                dkl[blk * F::DS + key] = d * 16777216.0f;
+                dkl[blk * F::DS + key] = d;
                 fa4_block(vr[it], blk, d, q);
                 *(uint4 *) (vl + F::voff(key) + blk * 16) = make_uint4(q[0], q[1], q[2], q[3]);
                 d   = live >> key & 1 ? d : 0.0f;
@@ -423,8 +398,8 @@ __global__ void __launch_bounds__(64 * W) k_fa4_dec(const FaArgs a) {
                     const fa4_f4 dk = *(const fa4_f4 *) (dkl + blk * F::DS + 16 * mt + 4 * q4);
 #pragma unroll
                     for (int p = QP - 1; p >= 0; --p) {
-                        const float  c   = c0[p][blk];
-                        const fa4_f4 acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, qb[p][blk], fa4_f4{ c, c, c, c }, 0, 0, 0);
+                        const fa4_f4 acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                            x, qb[p][blk], fa4_f4{ 0.0f, 0.0f, 0.0f, 0.0f }, 0, 0, 0);
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
                             t[r] = __builtin_fmaf(acc[r], dk[r], t[r]);
@@ -589,51 +564,98 @@ __global__ void __launch_bounds__(64 * W) k_fa4_dec(const FaArgs a) {
 }
 
 // The splits' partial results of a row: y = sum_i w_i o_i / sum_i w_i l_i with w_i =
-// exp2(m_i - max m). A wave per row, a lane per D / 64 columns.
+// exp2(m_i - max m). A workgroup per row: D / 4 lanes take a float4 of the columns, the groups of
+// them every SG-th split. The outputs of the first PRE splits of each group are loaded with the
+// (m, l), before the weights are known: one round of memory latency for up to SG * PRE splits.
+constexpr int FA4_MAX_SPLITS = 1024;
+
 template <int D>
-__global__ void __launch_bounds__(64) k_fa4_combine(const FaArgs a) {
-    constexpr int  C    = D / 64;
-    const int      lane = threadIdx.x;
-    const uint32_t rec  = blockIdx.x;
-    const uint32_t bg   = rec / (uint32_t) a.rows;
-    const int      row  = (int) (rec - bg * (uint32_t) a.rows);
-    const uint32_t b    = bg / (uint32_t) a.nkv;
-    const uint32_t g    = bg - b * (uint32_t) a.nkv;
-    const int      iq   = row / a.rk;
-    const int      h    = (int) g * a.rk + (row - iq * a.rk);
-    const float *  p    = a.ws + (int64_t) rec * a.splits * (D + 4);
-    float          m = -INFINITY, l = 0.0f, acc[C] = {};
-    for (int s0 = 0; s0 < a.splits; s0 += 64) {
-        const int   n  = a.splits - s0 < 64 ? a.splits - s0 : 64;
-        const int   s  = s0 + (lane < n ? lane : n - 1);
-        const float ms = lane < n ? p[(int64_t) s * (D + 4)] : -INFINITY;
-        const float ls = p[(int64_t) s * (D + 4) + 1];
-        const float mn = fmaxf(m, group_max<64>(ms));
-        const float al = m == mn ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
-        const float w  = ms == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ms - mn);
-        l              = __builtin_fmaf(l, al, group_sum<64>(w == 0.0f ? 0.0f : w * ls));
-        m              = mn;
+__global__ void __launch_bounds__(256) k_fa4_combine(const FaArgs a) {
+    constexpr int C4 = D / 4, SG = 256 / C4, PRE = 8;
+    __shared__ float                wsh[FA4_MAX_SPLITS];
+    __shared__ float                red[8];
+    __shared__ __align__(16) fa4_f4 part[SG][C4];
+    const int      tid = threadIdx.x, c = tid % C4, sg = tid / C4;
+    const uint32_t rec = blockIdx.x;
+    const uint32_t bg  = rec / (uint32_t) a.rows;
+    const int      row = (int) (rec - bg * (uint32_t) a.rows);
+    const uint32_t b   = bg / (uint32_t) a.nkv;
+    const uint32_t g   = bg - b * (uint32_t) a.nkv;
+    const int      iq = row / a.rk, h = (int) g * a.rk + (row - iq * a.rk), last = a.splits - 1;
+    const float *  p = a.ws + (int64_t) rec * a.splits * (D + 4);
+    fa4_f4         pv[PRE];
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-            acc[c] *= al;
+    for (int j = 0; j < PRE; ++j) {  // past the last split: the last one again, weight 0
+        const int s = sg + SG * j;
+        pv[j]       = *(const fa4_f4 *) (p + (int64_t) (s < last ? s : last) * (D + 4) + 4 + 4 * c);
+    }
+    float ml[FA4_MAX_SPLITS / 256], ll[FA4_MAX_SPLITS / 256], m = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < FA4_MAX_SPLITS / 256; ++i) {
+        const int    s = tid + 256 * i;
+        const float2 x = *(const float2 *) (p + (int64_t) (s < last ? s : last) * (D + 4));
+        ml[i]          = s <= last ? x.x : -INFINITY;
+        ll[i]          = x.y;
+        m              = fmaxf(m, ml[i]);
+    }
+    m = group_max<64>(m);
+    if ((tid & 63) == 0) {
+        red[tid >> 6] = m;
+    }
+    __syncthreads();
+    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+#pragma unroll
+    for (int i = 0; i < FA4_MAX_SPLITS / 256; ++i) {
+        const int   s = tid + 256 * i;
+        const float w = ml[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml[i] - m);
+        wsh[s]        = w;
+        l             = w == 0.0f ? l : __builtin_fmaf(w, ll[i], l);
+    }
+    l = group_sum<64>(l);
+    if ((tid & 63) == 0) {
+        red[4 + (tid >> 6)] = l;
+    }
+    __syncthreads();
+    l          = (red[4] + red[5]) + (red[6] + red[7]);
+    fa4_f4 acc = { 0.0f, 0.0f, 0.0f, 0.0f };
+#pragma unroll
+    for (int j = 0; j < PRE; ++j) {
+        const float w = wsh[sg + SG * j];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            acc[e] = w == 0.0f ? acc[e] : __builtin_fmaf(w, pv[j][e], acc[e]);
         }
-        for (int j = 0; j < n; ++j) {
-            const float   wj = __shfl(w, j, 64);
-            const float * op = p + (int64_t) (s0 + j) * (D + 4) + 4 + lane * C;
+    }
+    for (int s0 = SG * PRE + sg; s0 <= last; s0 += SG * PRE) {
 #pragma unroll
-            for (int c = 0; c < C; ++c) {
-                acc[c] = __builtin_fmaf(wj, op[c], acc[c]);
+        for (int j = 0; j < PRE; ++j) {
+            const int s = s0 + SG * j;
+            pv[j]       = *(const fa4_f4 *) (p + (int64_t) (s < last ? s : last) * (D + 4) + 4 + 4 * c);
+        }
+#pragma unroll
+        for (int j = 0; j < PRE; ++j) {
+            const int   s = s0 + SG * j;
+            const float w = s <= last ? wsh[s] : 0.0f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                acc[e] = w == 0.0f ? acc[e] : __builtin_fmaf(w, pv[j][e], acc[e]);
             }
         }
     }
-    char * yp = a.y + (int64_t) b * a.y3 + (int64_t) iq * a.y2 + (int64_t) h * a.y1;
+    part[sg][c] = acc;
+    __syncthreads();
+    if (tid < C4) {
+        fa4_f4 t = part[0][tid];
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-        const float v = acc[c] / l;  // no live key: 0 / 0
+        for (int q = 1; q < SG; ++q) {
+            t += part[q][tid];
+        }
+        t *= 1.0f / l;  // no live key: 0 * inf
+        char * yp = a.y + (int64_t) b * a.y3 + (int64_t) iq * a.y2 + (int64_t) h * a.y1;
         if (a.ty == MI_TYPE_F32) {
-            store_elem<MI_TYPE_F32>(yp + (size_t) (lane * C + c) * 4, v);
+            *(fa4_f4u *) (yp + 16 * tid) = t;
         } else {
-            store_elem<MI_TYPE_BF16>(yp + (size_t) (lane * C + c) * 2, v);
+            *(fa4_u2u *) (yp + 8 * tid) = fa4_u2u{ pack_bf16x2(t[0], t[1]), pack_bf16x2(t[2], t[3]) };
         }
     }
 }
@@ -1186,9 +1208,7 @@ void flash_attn_q4_plan(FaArgs & a, int D) {
     a.rblocks = (a.rows + 15) / 16;
     a.splits  = 1;
     a.ngq     = (a.n_q + 15) / 16;
-    const int     tk    = D == 256 ? 32 : 64;
-    const int64_t tiles = ((int64_t) a.n_kv + tk - 1) / tk;
-    if (a.nb == 0 || a.rows == 0 || tiles == 0) {
+    if (a.nb == 0 || a.rows == 0 || a.n_kv == 0) {
         return;
     }
     if (a.n_kv > 1 << 27 || a.k1 >= 1 << 25 || a.v1 >= 1 << 25) {
@@ -1196,7 +1216,9 @@ void flash_attn_q4_plan(FaArgs & a, int D) {
         return;
     }
     a.mfma = a.rows > FA4_DEC_ROWS && a.ngq <= 65535 && (int64_t) a.nb * a.nh <= 65535;
-    int64_t items, want, most, least = 1;
+    int64_t       items, want, most, least = 1;
+    const int     tk    = a.mfma ? (D == 256 ? 32 : 64) : (D == 64 ? 64 : 32);  // keys per tile
+    const int64_t tiles = ((int64_t) a.n_kv + tk - 1) / tk;
     if (a.mfma) {
         // the workspace is sized without y: its type (rows per workgroup) must not change the splits
         a.rblocks = (a.rows + 127) / 128;
@@ -1206,14 +1228,15 @@ void flash_attn_q4_plan(FaArgs & a, int D) {
         least     = (tiles + FA4_PRE_TILES - 1) / FA4_PRE_TILES;
     } else {
         items = (int64_t) a.nb * a.nkv * a.rblocks;
-        // enough waves for 16 per CU, at most one tile each
-        want = ((int64_t) num_cus() * 16 / FA4_W + items - 1) / items;
-        most = (tiles + FA4_W - 1) / FA4_W;
+        want = (int64_t) num_cus() * (D == 256 ? 1 : 3) / items;
+        most = (tiles + 2 * FA4_W - 1) / (2 * FA4_W);
     }
+    most     = most < FA4_MAX_SPLITS ? most : FA4_MAX_SPLITS;
     want     = want < most ? want : most;
     a.splits = (int) (want < least ? least : want);
-    if (items * a.splits >= ((int64_t) 1 << 31)) {
-        a.splits = 0;  // more workgroups than a grid has
+    if (a.splits > FA4_MAX_SPLITS || items * a.splits >= ((int64_t) 1 << 31)) {
+        a.splits = 0;  // more than the merge or a grid takes
+        return;
     }
     if (a.mfma) {
         const int bq = fa4_bq(D, a.ty == MI_TYPE_F32);
@@ -1252,7 +1275,7 @@ static void launch_dec(const FaArgs & a, hipStream_t s) {
         MI_LAUNCH((k_fa4_dec<D, OS, 2, FA4_W>), grid, wg, 0, s, a);
     }
     if (a.splits > 1) {
-        MI_LAUNCH((k_fa4_combine<D>), dim3((uint32_t) (a.nb * a.nkv * a.rows)), dim3(64), 0, s, a);
+        MI_LAUNCH((k_fa4_combine<D>), dim3((uint32_t) (a.nb * a.nkv * a.rows)), dim3(256), 0, s, a);
     }
 }
 
