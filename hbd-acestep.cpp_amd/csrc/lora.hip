@@ -41,38 +41,36 @@ __device__ __forceinline__ LrSplit lr_split(const float * x) {
 // 8 weights as one or two bf16 parts
 template <int WT> struct LrW;
 template <> struct LrW<MI_TYPE_BF16> {
+    uint4                           raw;
     lr_b8                           p;
-    __device__ __forceinline__ void set(const uint4 & v) { p = __builtin_bit_cast(lr_b8, v); }
-    __device__ __forceinline__ lr_f4 mul(const LrSplit & x, lr_f4 c, bool first) const {
-        // weights as A, x as B, or the other way round
+    __device__ __forceinline__ void split() { p = __builtin_bit_cast(lr_b8, raw); }
+    __device__ __forceinline__ lr_f4 mul(const LrSplit & x, lr_f4 c) const {
 #pragma unroll
         for (int i = 2; i >= 0; --i) {
-            c = first ? __builtin_amdgcn_mfma_f32_16x16x32_bf16(p, x.p[i], c, 0, 0, 0)
-                      : __builtin_amdgcn_mfma_f32_16x16x32_bf16(x.p[i], p, c, 0, 0, 0);
+            c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x.p[i], p, c, 0, 0, 0);
         }
         return c;
     }
 };
 template <> struct LrW<MI_TYPE_F16> {
+    uint4                           raw;
     lr_b8                           hi, lo;
-    __device__ __forceinline__ void set(const uint4 & v) {
+    __device__ __forceinline__ void split() {
         float f[8];
-        unpack16<MI_TYPE_F16>(v, f);
+        unpack16<MI_TYPE_F16>(raw, f);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             hi[e] = (__bf16) f[e];
             lo[e] = (__bf16) (f[e] - (float) hi[e]);  // 11 significant bits less 8: exact
         }
     }
-    __device__ __forceinline__ lr_f4 mul(const LrSplit & x, lr_f4 c, bool first) const {
+    __device__ __forceinline__ lr_f4 mul(const LrSplit & x, lr_f4 c) const {
 #pragma unroll
         for (int i = 2; i >= 0; --i) {
             if (i < 2) {
-                c = first ? __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, x.p[i], c, 0, 0, 0)
-                          : __builtin_amdgcn_mfma_f32_16x16x32_bf16(x.p[i], lo, c, 0, 0, 0);
+                c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x.p[i], lo, c, 0, 0, 0);
             }
-            c = first ? __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, x.p[i], c, 0, 0, 0)
-                      : __builtin_amdgcn_mfma_f32_16x16x32_bf16(x.p[i], hi, c, 0, 0, 0);
+            c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x.p[i], hi, c, 0, 0, 0);
         }
         return c;
     }
@@ -129,12 +127,13 @@ __global__ void __launch_bounds__(256) k_lora_down(const LoraArgs a) {
 #pragma unroll
             for (int i = 0; i < NR; ++i) {
                 const lr_u4a v = *(const lr_u4a *) (wp[i] + (int64_t) s * 64);
-                w[i].set(make_uint4(v.x, v.y, v.z, v.w));
+                w[i].raw = make_uint4(v.x, v.y, v.z, v.w);
             }
             const LrSplit xs = lr_split(xv);
 #pragma unroll
             for (int i = 0; i < NR; ++i) {
-                c[i] = w[i].mul(xs, c[i], false);
+                w[i].split();
+                c[i] = w[i].mul(xs, c[i]);
             }
         }
         __syncthreads();  // the previous adapter's sums are read
@@ -164,121 +163,198 @@ __global__ void __launch_bounds__(256) k_lora_down(const LoraArgs a) {
     }
 }
 
-// y = y0 + B (scale h). A workgroup: 16 rows of x (blockIdx.x) and 64 NT columns of y (y); a
-// wave 16 NT of them. h is summed over the key shares, scaled and split once, into LDS.
-template <int WT, int NT>
+// y = y0 + B (scale h). A workgroup: 16 TT rows of x (blockIdx.x) and every gridDim.y-th block of
+// 64 NT columns of y, a wave 16 NT of them. h is summed over the key shares, scaled and split
+// once, into LDS; a block's y0 is loaded under the block before it. RS: steps of 32 ranks; U:
+// adapters whose weights are loaded before the first is multiplied.
+// Column c of product i is column NT c + i of the wave's: a lane holds NT consecutive columns of
+// 4 rows, and with NT 4 a load or store of y covers 256 consecutive bytes of a row (products of
+// 16 consecutive columns each: 64, and 167 us instead of 138 for 4005 x 19456 at rank 32).
+template <int WT, int NT, int TT, int RS, int U>
 __global__ void __launch_bounds__(256) k_lora_up(const LoraArgs a) {
-    extern __shared__ __align__(16) __bf16 hs[];  // [3][16][rq], rq = rank padded to 32, + 8
+    static_assert(NT == 1 || NT == 4, "a dword or a float4 of y per lane and row");
+    constexpr int RQ = RS * 32 + 8;  // row of h in LDS: 16 rows on distinct banks
+    constexpr int R  = 16 * TT;
+    typedef float lr_y __attribute__((ext_vector_type(NT), aligned(4)));
+    __shared__ __align__(16) __bf16 hs[3 * R * RQ];
     const int      lane = threadIdx.x & 63, c16 = lane & 15, q4 = lane >> 4;
     const int      wv   = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t t0   = blockIdx.x * 16;
-    const int      rk32 = (int) ((a.r + 31) / 32), rq = rk32 * 32 + 8;
-    const int32_t  id   = lr_id(a, t0 + c16);
-    for (int i = threadIdx.x; i < 16 * rk32 * 32; i += 256) {
-        const int      t = i / (rk32 * 32), r = i - t * rk32 * 32;
-        const int32_t  it = lr_id(a, t0 + t);
-        float          v  = 0.0f;
+    const uint32_t t0   = blockIdx.x * R;
+    const int32_t  idl  = lr_id(a, t0 + (lane < R ? lane : R));  // lanes 0 .. R - 1: the rows' adapters
+    const uint64_t rows = __builtin_amdgcn_ballot_w64(idl >= 0 && lane < R);
+    int32_t        id[TT][4];
+#pragma unroll
+    for (int tt = 0; tt < TT; ++tt) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            id[tt][e] = __shfl(idl, tt * 16 + 4 * q4 + e, 64);
+        }
+    }
+    // element (row tt * 16 + 4 q4 + e, columns n ..); rows past the last: the last one again
+    auto row = [&](int tt, int e) -> int64_t {
+        const uint32_t t = t0 + tt * 16 + 4 * q4 + e;
+        return t < a.m ? t : a.m - 1;
+    };
+    lr_y acc[TT][4], nxt[TT][4];
+    auto load = [&](uint32_t n0) {  // columns past the last: the last ones again
+        const uint32_t n = n0 + NT * c16;
+        const int64_t  c = (int64_t) (n + NT <= a.n ? n : a.n - NT) * 4;
+#pragma unroll
+        for (int tt = 0; tt < TT; ++tt) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                nxt[tt][e] = *(const lr_y *) (a.y0 + row(tt, e) * a.y01 + c);
+            }
+        }
+    };
+    uint32_t n0 = (blockIdx.y * 4 + wv) * (16 * NT);
+    load(n0);
+    for (int i = threadIdx.x; i < R * RS * 32; i += 256) {
+        const int     t = i / (RS * 32), r = i - t * RS * 32;
+        const int32_t it = lr_id(a, t0 + t);
+        float         v  = 0.0f;
         if (it >= 0 && r < (int) a.r) {
-            for (uint32_t s = 0; s < a.ks; ++s) {
-                v += a.h[((int64_t) s * a.m + t0 + t) * a.rp + r];
+            const float * hp = a.h + (int64_t) (t0 + t) * a.rp + r;
+            const int64_t st = (int64_t) a.m * a.rp;
+            uint32_t      s  = 0;
+            for (; s + 4 <= a.ks; s += 4) {
+                const float p0 = hp[s * st], p1 = hp[(s + 1) * st], p2 = hp[(s + 2) * st], p3 = hp[(s + 3) * st];
+                v += (p0 + p1) + (p2 + p3);
+            }
+            for (; s < a.ks; ++s) {
+                v += hp[s * st];
             }
             v *= a.scales ? *(const float *) (a.scales + (int64_t) it * a.s0) : 1.0f;
         }
         const __bf16 p0 = (__bf16) v;
         const float  r0 = v - (float) p0;
         const __bf16 p1 = (__bf16) r0;
-        hs[t * rq + r]                = p0;
-        hs[(16 + t) * rq + r]         = p1;
-        hs[(32 + t) * rq + r]         = (__bf16) (r0 - (float) p1);
+        hs[t * RQ + r]           = p0;
+        hs[(R + t) * RQ + r]     = p1;
+        hs[(2 * R + t) * RQ + r] = (__bf16) (r0 - (float) p1);
     }
     __syncthreads();
-    const uint32_t n0 = (blockIdx.y * 4 + wv) * (16 * NT);
-    if (n0 >= a.n) {
-        return;
-    }
-    const uint32_t tr = t0 + c16 < a.m ? t0 + c16 : a.m - 1;
-    const char *   y0 = a.y0 + (int64_t) tr * a.y01;
-    lr_f4          acc[NT];
+    const bool vec = a.r % 8 == 0;
+    for (; n0 < a.n; n0 += gridDim.y * (64 * NT)) {
 #pragma unroll
-    for (int i = 0; i < NT; ++i) {
-        const uint32_t n = n0 + 16 * i + 4 * q4;
-        if (n + 4 <= a.n) {
-            acc[i] = *(const lr_f4a *) (y0 + (int64_t) n * 4);
-        } else {
+        for (int tt = 0; tt < TT; ++tt) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                acc[i][e] = n + e < a.n ? *(const float *) (y0 + (int64_t) (n + e) * 4) : 0.0f;
+                acc[tt][e] = nxt[tt][e];
             }
         }
-    }
-    uint64_t todo = __builtin_amdgcn_ballot_w64(id >= 0) & 0xffffu;
-    while (todo) {
-        const int32_t  cur  = __builtin_amdgcn_readlane(id, __builtin_ctzll(todo));
-        const uint64_t mine = __builtin_amdgcn_ballot_w64(id == cur) & 0xffffu;
-        todo &= ~mine;
-        const char * bp[NT];
-        lr_f4        c[NT];
+        load(n0 + gridDim.y * (64 * NT));
+        uint64_t todo = rows;
+        while (todo) {
+            int32_t cur[U];
+            LrW<WT> w[U][RS][NT];
 #pragma unroll
-        for (int i = 0; i < NT; ++i) {
-            const uint32_t n = n0 + 16 * i + c16;
-            bp[i] = a.b + (int64_t) cur * a.b2 + (int64_t) (n < a.n ? n : a.n - 1) * a.b1;
-            c[i]  = lr_f4{ 0.0f, 0.0f, 0.0f, 0.0f };
-        }
-        for (int s = 0; s < rk32; ++s) {
-            LrSplit h;
+            for (int u = 0; u < U; ++u) {
+                cur[u] = -2;  // no row's
+                if (todo) {
+                    cur[u] = __builtin_amdgcn_readlane(idl, __builtin_ctzll(todo));
+                    todo &= ~__builtin_amdgcn_ballot_w64(idl == cur[u]);
+                    const char * bp = a.b + (int64_t) cur[u] * a.b2 + q4 * 16;
 #pragma unroll
-            for (int p = 0; p < 3; ++p) {
-                h.p[p] = *(const lr_b8 *) (hs + (16 * p + c16) * rq + s * 32 + 8 * q4);
-            }
-            const int r0 = s * 32 + 8 * q4;
-            LrW<WT>   w[NT];
+                    for (int i = 0; i < NT; ++i) {
+                        const uint32_t n = n0 + NT * c16 + i;
+                        const char *   p = bp + (int64_t) (n < a.n ? n : a.n - 1) * a.b1;
 #pragma unroll
-            for (int i = 0; i < NT; ++i) {
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (r0 + 8 <= (int) a.r) {
-                    const lr_u4a x = *(const lr_u4a *) (bp[i] + r0 * 2);
-                    v              = make_uint4(x.x, x.y, x.z, x.w);
-                } else if (r0 < (int) a.r) {
-                    uint16_t x[8];
+                        for (int s = 0; s < RS; ++s) {
+                            const int r0 = s * 32 + 8 * q4;
+                            uint4     v  = make_uint4(0, 0, 0, 0);
+                            if (r0 + 8 <= (int) a.r) {
+                                const lr_u4a x = *(const lr_u4a *) (p + s * 64);
+                                v              = make_uint4(x.x, x.y, x.z, x.w);
+                            } else if (!vec && r0 < (int) a.r) {
+                                uint16_t x[8];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        x[e] = r0 + e < (int) a.r ? *(const uint16_t *) (bp[i] + (r0 + e) * 2) : 0;
+                                for (int e = 0; e < 8; ++e) {
+                                    x[e] = r0 + e < (int) a.r ? *(const uint16_t *) (p + s * 64 + e * 2) : 0;
+                                }
+                                v = make_uint4(x[0] | (uint32_t) x[1] << 16, x[2] | (uint32_t) x[3] << 16,
+                                               x[4] | (uint32_t) x[5] << 16, x[6] | (uint32_t) x[7] << 16);
+                            }
+                            w[u][s][i].raw = v;
+                        }
                     }
-                    v = make_uint4(x[0] | (uint32_t) x[1] << 16, x[2] | (uint32_t) x[3] << 16,
-                                   x[4] | (uint32_t) x[5] << 16, x[6] | (uint32_t) x[7] << 16);
                 }
-                w[i].set(v);
             }
 #pragma unroll
-            for (int i = 0; i < NT; ++i) {
-                c[i] = w[i].mul(h, c[i], true);
+            for (int u = 0; u < U; ++u) {
+                if (cur[u] == -2) {
+                    break;
+                }
+                lr_f4 c[TT][NT] = {};
+#pragma unroll
+                for (int s = 0; s < RS; ++s) {
+                    LrSplit h[TT];
+#pragma unroll
+                    for (int tt = 0; tt < TT; ++tt) {
+#pragma unroll
+                        for (int p = 0; p < 3; ++p) {
+                            h[tt].p[p] = *(const lr_b8 *) (hs + (R * p + tt * 16 + c16) * RQ + s * 32 + 8 * q4);
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < NT; ++i) {
+                        w[u][s][i].split();
+#pragma unroll
+                        for (int tt = 0; tt < TT; ++tt) {
+                            c[tt][i] = w[u][s][i].mul(h[tt], c[tt][i]);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int tt = 0; tt < TT; ++tt) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const bool mine = id[tt][e] == cur[u];
+#pragma unroll
+                        for (int i = 0; i < NT; ++i) {
+                            acc[tt][e][i] = mine ? acc[tt][e][i] + c[tt][i][e] : acc[tt][e][i];
+                        }
+                    }
+                }
             }
         }
-        if (id == cur) {
+        const uint32_t n = n0 + NT * c16;
+        if (n + NT <= a.n) {
 #pragma unroll
-            for (int i = 0; i < NT; ++i) {
-                acc[i] += c[i];
+            for (int tt = 0; tt < TT; ++tt) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (t0 + tt * 16 + 4 * q4 + e < a.m) {
+                        *(lr_y *) (a.y + row(tt, e) * a.y1 + (int64_t) n * 4) = acc[tt][e];
+                    }
+                }
             }
         }
     }
-    if (t0 + c16 >= a.m) {
+}
+
+// The columns past the last whole 4 (at most 3): a thread each, in fp32, the ranks in order.
+__global__ void __launch_bounds__(256) k_lora_up_rest(const LoraArgs a, int f16) {
+    const uint32_t left = a.n & 3u, i = blockIdx.x * 256 + threadIdx.x;
+    if (i >= a.m * left) {
         return;
     }
-    char * y = a.y + (int64_t) tr * a.y1;
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-        const uint32_t n = n0 + 16 * i + 4 * q4;
-        if (n + 4 <= a.n) {
-            *(lr_f4a *) (y + (int64_t) n * 4) = acc[i];
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (n + e < a.n) {
-                    *(float *) (y + (int64_t) (n + e) * 4) = acc[i][e];
-                }
+    const uint32_t t = i / left, n = a.n - left + (i - t * left);
+    const int32_t  id = lr_id(a, t);
+    float          v  = *(const float *) (a.y0 + (int64_t) t * a.y01 + (int64_t) n * 4);
+    if (id >= 0) {
+        const char * bp = a.b + (int64_t) id * a.b2 + (int64_t) n * a.b1;
+        float        c  = 0.0f;
+        for (uint32_t r = 0; r < a.r; ++r) {
+            float h = 0.0f;
+            for (uint32_t s = 0; s < a.ks; ++s) {
+                h += a.h[((int64_t) s * a.m + t) * a.rp + r];
             }
+            c = __builtin_fmaf(h, f16 ? load_elem<MI_TYPE_F16>(bp + r * 2) : load_elem<MI_TYPE_BF16>(bp + r * 2), c);
         }
+        v += c * (a.scales ? *(const float *) (a.scales + (int64_t) id * a.s0) : 1.0f);
     }
+    *(float *) (a.y + (int64_t) t * a.y1 + (int64_t) n * 4) = v;
 }
 
 void lora_plan(LoraArgs & a) {
@@ -304,6 +380,24 @@ template <int WT, int NR> static void launch_down(const LoraArgs & a, hipStream_
     MI_LAUNCH((k_lora_down<WT, NR>), dim3((a.m + 15) / 16, a.ks, blocks * a.slots), dim3(256), 0, s, a);
 }
 
+// many rows of at least 4 columns: 4 columns of y a lane
+static bool lora_wide(const LoraArgs & a) {
+    return a.m > 64 && a.n >= 4;
+}
+
+template <int WT, int RS> static void launch_up(const LoraArgs & a, hipStream_t s) {
+    if (lora_wide(a)) {
+        // rows in tiles of 32 (16 at high ranks), column blocks of 256 over enough workgroups for 8 per CU
+        constexpr int  TT    = RS < 8 ? 2 : 1;
+        const uint32_t tiles = (a.m + 16 * TT - 1) / (16 * TT), blocks = (a.n + 255) / 256;
+        const uint32_t want  = ((uint32_t) num_cus() * 8 + tiles - 1) / tiles;
+        MI_LAUNCH((k_lora_up<WT, 4, TT, RS, 1>), dim3(tiles, want < blocks ? want : blocks), dim3(256), 0, s, a);
+    } else {
+        MI_LAUNCH((k_lora_up<WT, 1, 1, RS, RS < 4 ? 4 : RS < 8 ? 2 : 1>), dim3((a.m + 15) / 16, (a.n + 63) / 64),
+                  dim3(256), 0, s, a);
+    }
+}
+
 template <int WT> static void launch_w(const LoraArgs & a, hipStream_t s) {
     if (a.rp <= 16) {
         launch_down<WT, 1>(a, s);
@@ -312,8 +406,17 @@ template <int WT> static void launch_w(const LoraArgs & a, hipStream_t s) {
     } else {
         launch_down<WT, 4>(a, s);
     }
-    const size_t lb = (size_t) 48 * ((a.r + 31) / 32 * 32 + 8) * 2;
-    MI_LAUNCH((k_lora_up<WT, 4>), dim3((a.m + 15) / 16, (a.n + 255) / 256), dim3(256), lb, s, a);
+    switch ((a.r + 31) / 32) {
+        case 1: launch_up<WT, 1>(a, s); break;
+        case 2: launch_up<WT, 2>(a, s); break;
+        case 3:
+        case 4: launch_up<WT, 4>(a, s); break;
+        default: launch_up<WT, 8>(a, s); break;
+    }
+    if (lora_wide(a) && a.n % 4 != 0) {
+        MI_LAUNCH(k_lora_up_rest, dim3((uint32_t) (((uint64_t) a.m * (a.n & 3u) + 255) / 256)), dim3(256), 0, s, a,
+                  WT == MI_TYPE_F16 ? 1 : 0);
+    }
 }
 
 int launch_lora(const LoraArgs & a, int type, hipStream_t s) {
