@@ -210,22 +210,26 @@ __global__ void __launch_bounds__(256) k_lora_up(const LoraArgs a) {
     uint32_t n0 = (blockIdx.y * 4 + wv) * (16 * NT);
     load(n0);
     for (int i = threadIdx.x; i < R * RS * 32; i += 256) {
-        const int     t = i / (RS * 32), r = i - t * RS * 32;
-        const int32_t it = lr_id(a, t0 + t);
-        float         v  = 0.0f;
-        if (it >= 0 && r < (int) a.r) {
-            const float * hp = a.h + (int64_t) (t0 + t) * a.rp + r;
-            const int64_t st = (int64_t) a.m * a.rp;
-            uint32_t      s  = 0;
-            for (; s + 4 <= a.ks; s += 4) {
-                const float p0 = hp[s * st], p1 = hp[(s + 1) * st], p2 = hp[(s + 2) * st], p3 = hp[(s + 3) * st];
-                v += (p0 + p1) + (p2 + p3);
+        const int      t = i / (RS * 32), r = i - t * RS * 32;
+        const int32_t  it  = __shfl(idl, t, 64);
+        const bool     on  = it >= 0 && r < (int) a.r;
+        const uint32_t tr  = t0 + t < a.m ? t0 + t : a.m - 1;
+        const float *  hp  = a.h + (int64_t) tr * a.rp + (r < (int) a.r ? r : 0);
+        const int64_t  st  = (int64_t) a.m * a.rp;
+        const float    sc  = a.scales && on ? *(const float *) (a.scales + (int64_t) it * a.s0) : 1.0f;
+        float          v   = 0.0f;
+        for (uint32_t s = 0; s < a.ks; s += 16) {  // 16 shares in flight; rows without an adapter hold anything
+            float p[16];
+#pragma unroll
+            for (int q = 0; q < 16; ++q) {
+                p[q] = hp[(s + q < a.ks ? s + q : a.ks - 1) * st];
             }
-            for (; s < a.ks; ++s) {
-                v += hp[s * st];
+#pragma unroll
+            for (int q = 0; q < 16; ++q) {
+                v += s + q < a.ks ? p[q] : 0.0f;
             }
-            v *= a.scales ? *(const float *) (a.scales + (int64_t) it * a.s0) : 1.0f;
         }
+        v = on ? v * sc : 0.0f;
         const __bf16 p0 = (__bf16) v;
         const float  r0 = v - (float) p0;
         const __bf16 p1 = (__bf16) r0;
