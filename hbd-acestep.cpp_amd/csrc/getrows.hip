@@ -273,15 +273,17 @@ __global__ void __launch_bounds__(256) k_get_rows_q8_0_flat(const GetRowsArgs a,
     }
 }
 
-// Q4_0 rows: y = (q - 8) * d, exact in fp32 (4 + 11 significant bits). Flat, as
-// above, but a thread makes 2 * OPS outputs from one load of OPS bytes: the low
-// nibbles are elements e .. e + OPS - 1 of a block's first half, the high ones
-// the same of its second half, so every byte is read once.
+// Q4_0 rows: y = (q - 8) * d, exact in fp32 (4 + 11 significant bits). Flat, as above: a thread
+// makes one 16-byte store per step, whole lines per store instruction, from OPS consecutive
+// nibbles of one half of a block (one load at the levels' 2-byte alignment; the other half's
+// thread reads the same bytes again, from the cache).
+typedef uint32_t gr_u2 __attribute__((ext_vector_type(2), aligned(2)));
+typedef uint32_t gr_u1 __attribute__((aligned(2)));
+
 template <int TO, int U>
 __global__ void __launch_bounds__(256) k_get_rows_q4_0_flat(const GetRowsArgs a, FastDiv per_row, uint32_t nchunks) {
     constexpr int  EO  = TT<TO>::ES;
-    constexpr int  OPS = 16 / EO;   // bytes of quants per thread, outputs per store
-    constexpr int  CPB = 16 / OPS;  // threads per block
+    constexpr int  OPS = 16 / EO;
     const uint32_t c0  = blockIdx.x * (256 * U) + threadIdx.x;
     uint32_t       i[U];
     int            o[U];
@@ -290,19 +292,23 @@ __global__ void __launch_bounds__(256) k_get_rows_q4_0_flat(const GetRowsArgs a,
     for (int u = 0; u < U; ++u) {
         const uint32_t c = c0 + 256 * u < nchunks ? c0 + 256 * u : nchunks - 1;  // clamped: loads stay in bounds
         i[u]             = per_row.div(c);
-        o[u]             = (int) (c - i[u] * per_row.d);
+        o[u]             = (int) (c - i[u] * per_row.d) * OPS;
         r[u]             = a.ids[(int64_t) i[u] * a.ids_stride];
     }
-    uint16_t dh[U], q[U][OPS / 2];
+    uint16_t dh[U];
+    uint32_t q[U][2];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        const bool       ok = r[u] >= 0 && r[u] < a.n_rows;
-        const char *     bp = a.table + (ok ? r[u] : 0) * a.tnb1 + (int64_t) (o[u] / CPB) * 18;
-        const uint16_t * qp = (const uint16_t *) (bp + 2 + (o[u] % CPB) * OPS);
-        dh[u]               = *(const uint16_t *) bp;
-#pragma unroll
-        for (int h = 0; h < OPS / 2; ++h) {
-            q[u][h] = qp[h];
+        const bool   ok = r[u] >= 0 && r[u] < a.n_rows;
+        const char * bp = a.table + (ok ? r[u] : 0) * a.tnb1 + (int64_t) (o[u] >> 5) * 18;
+        const char * qp = bp + 2 + (o[u] & 15);
+        dh[u]           = *(const uint16_t *) bp;
+        if constexpr (OPS == 8) {
+            const gr_u2 v = *(const gr_u2 *) qp;
+            q[u][0]       = v.x;
+            q[u][1]       = v.y;
+        } else {
+            q[u][0] = *(const gr_u1 *) qp;
         }
     }
 #pragma unroll
@@ -315,16 +321,13 @@ __global__ void __launch_bounds__(256) k_get_rows_q4_0_flat(const GetRowsArgs a,
             atomicAdd(a.d_err, 1);
         }
         const float d = (float) __builtin_bit_cast(_Float16, dh[u]);
-        float       lo[OPS], hi[OPS];
+        float       f[OPS];
 #pragma unroll
         for (int k = 0; k < OPS; ++k) {
-            const uint32_t b = (uint32_t) q[u][k / 2] >> (8 * (k % 2));
-            lo[k]            = bad ? 0.0f : (float) ((int32_t) (b & 15u) - 8) * d;
-            hi[k]            = bad ? 0.0f : (float) ((int32_t) (b >> 4 & 15u) - 8) * d;
+            const uint32_t n = q[u][k / 4] >> (8 * (k % 4) + (o[u] & 16 ? 4 : 0)) & 15u;
+            f[k]             = bad ? 0.0f : (float) ((int32_t) n - 8) * d;
         }
-        char * yp = a.y + (int64_t) i[u] * a.ynb1 + (int64_t) ((o[u] / CPB) * 32 + (o[u] % CPB) * OPS) * EO;
-        store_vec<TO, OPS>(yp, lo);
-        store_vec<TO, OPS>(yp + 16 * EO, hi);
+        store_vec<TO, OPS>(a.y + (int64_t) i[u] * a.ynb1 + (int64_t) o[u] * EO, f);
     }
 }
 
@@ -420,12 +423,12 @@ static int launch_to(const GetRowsArgs & a, int ttype, bool fast, bool lds, hipS
             }
             case MI_TYPE_Q4_0: {
                 constexpr int      OPS     = 16 / TT<TO>::ES;
-                constexpr uint32_t per_wg  = 256 * MI_GR_FLAT_U / 2;  // half as many: a chunk is two stores
-                const uint64_t     nchunks = (uint64_t) a.n_ids * (uint64_t) (a.n / (2 * OPS));
+                constexpr uint32_t per_wg  = 256 * MI_GR_FLAT_U;
+                const uint64_t     nchunks = (uint64_t) a.n_ids * (uint64_t) (a.n / OPS);
                 if (a.n_rows > 0 && nchunks < (1ull << 31)) {  // an invalid id loads from row 0
-                    MI_LAUNCH((k_get_rows_q4_0_flat<TO, MI_GR_FLAT_U / 2>),
+                    MI_LAUNCH((k_get_rows_q4_0_flat<TO, MI_GR_FLAT_U>),
                                        dim3((uint32_t) ((nchunks + per_wg - 1) / per_wg)), dim3(256), 0, s, a,
-                                       FastDiv((uint32_t) (a.n / (2 * OPS))), (uint32_t) nchunks);
+                                       FastDiv((uint32_t) (a.n / OPS)), (uint32_t) nchunks);
                     return MI_OK;
                 }
                 break;

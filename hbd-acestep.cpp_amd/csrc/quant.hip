@@ -284,6 +284,8 @@ __global__ void __launch_bounds__(256) k_row_q8_lds(const RowCopy K, const RowCo
     }
 }
 
+typedef uint32_t q4_u2 __attribute__((ext_vector_type(2), aligned(2)));  // 8 bytes of levels in an 18-byte block
+
 // Q4_0 destinations, staged as k_row_q8_lds: a wave's tile of 32 consecutive
 // blocks comes into LDS by lane-contiguous 16-byte loads, then a lane pair
 // quantizes each block, the first lane elements 0-15 and the second 16-31. Byte j
@@ -363,11 +365,7 @@ __global__ void __launch_bounds__(256) k_row_q4_lds(const RowCopy K, const RowCo
     const uint32_t b0 = sub ? oth[2] | own[2] << 4 : own[0] | oth[0] << 4;
     const uint32_t b1 = sub ? oth[3] | own[3] << 4 : own[1] | oth[1] << 4;
     char *         bp = drow + (size_t) bi * 18;
-    uint16_t *     qp = (uint16_t *) (bp + 2 + sub * 8);  // 2-byte aligned
-    qp[0]             = (uint16_t) (b0 & 0xffffu);
-    qp[1]             = (uint16_t) (b0 >> 16);
-    qp[2]             = (uint16_t) (b1 & 0xffffu);
-    qp[3]             = (uint16_t) (b1 >> 16);
+    *(q4_u2 *) (bp + 2 + sub * 8) = q4_u2{ b0, b1 };
     if (sub == 0) {
         *(uint16_t *) bp = f32_to_f16_bits(d);
     }
