@@ -1,5 +1,5 @@
 """One Qwen3 decoder layer, every op on the device, with Q8_0 weights and a
-Q8_0 or F16 KV cache: batched decode (Qwen3Layer.forward, qw3lm_forward_batch,
+Q8_0, Q4_0 or F16 KV cache: batched decode (Qwen3Layer.forward, qw3lm_forward_batch,
 qwen3-lm.h:626-741) and prefill (Qwen3Layer.prefill, qw3lm_forward,
 qwen3-lm.h:429-549 with qw3lm_build_attn, 330-424). Decode:
 
@@ -33,7 +33,16 @@ kv_pos[b] + t and is stored at that slot of set s0 + b (qwen3-lm.h:396-406),
 and attention reads the first kv_len = max_b(kv_pos[b] + S) slots under the
 causal mask (N, 1, S, kv_len) F16, 0 for slots <= kv_pos[b] + t and -inf
 after (qwen3-lm.h:523-533): q (N, Nh, S, D) is a strided view of the roped q
-rows, as ggml's permute makes it (qwen3-lm.h:380)."""
+rows, as ggml's permute makes it (qwen3-lm.h:380).
+
+A layer given `adapters` adds each row's own low-rank update to the products
+that have one, y + scales[id] * B[id] (A[id] x), where a call names the rows'
+adapters; those products then run as the norm (or swiglu), the product and the
+update, since the fused calls keep no x. Calls that name none run as above.
+
+Qwen3Head is what follows the last layer in a decode step: the final norm and
+the vocabulary product, then the requests' penalties, biases and grammars on
+the logits."""
 from __future__ import annotations
 
 import math
@@ -66,8 +75,10 @@ def causal_mask(kv_pos, S: int, kv_len: int) -> DTensor:
 class Qwen3Layer:
     def __init__(self, w_qkv, w_o, w_gate_up, w_down, in_norm_w, post_norm_w, q_norm_w, k_norm_w, H: int, Nh: int,
                  Nkv: int, D: int, I: int, max_seq: int, n_sets: int, kv_type: str = "q8_0", eps: float = 1e-6,
-                 rope_theta: float = 1e6, clamp_fp16: bool = False, stream=None):
-        """w_*: Q8 weights in the GGUF layout (repacked here once); norms: F32 DTensors."""
+                 rope_theta: float = 1e6, clamp_fp16: bool = False, stream=None, adapters=None, adapter_scales=None):
+        """w_*: Q8 weights in the GGUF layout (repacked here once); norms: F32 DTensors.
+        adapters: {"qkv" | "o" | "gu" | "down": (A (n, r, k), B (n, n_out, r))} bf16 or f16, with
+        adapter_scales F32 (n,) or None (1)."""
         self.H, self.Nh, self.Nkv, self.D, self.I = H, Nh, Nkv, D, I
         self.eps, self.theta, self.stream = eps, rope_theta, stream
         self.clamp_fp16 = bool(clamp_fp16)
@@ -75,15 +86,19 @@ class Qwen3Layer:
                   for name, w in (("qkv", w_qkv), ("o", w_o), ("gu", w_gate_up), ("down", w_down))}
         self.in_norm_w, self.post_norm_w = in_norm_w, post_norm_w
         self.q_norm_w, self.k_norm_w = q_norm_w, k_norm_w
+        self.adapters, self.adapter_scales = dict(adapters or {}), adapter_scales
+        if not set(self.adapters) <= set(self.w):
+            raise ValueError("adapters: qkv, o, gu, down")
         self.kv_type = kv_type
-        if kv_type == "q8_0":
-            self.k_cache = ops.Q8(DTensor.zeros((n_sets, Nkv, max_seq, D // 32 * 34), "u8"))
-            self.v_cache = ops.Q8(DTensor.zeros((n_sets, Nkv, max_seq, D // 32 * 34), "u8"))
+        if kv_type in ("q8_0", "q4_0"):
+            wrap, nb = (ops.Q8, 34) if kv_type == "q8_0" else (ops.Q4, 18)
+            self.k_cache = wrap(DTensor.zeros((n_sets, Nkv, max_seq, D // 32 * nb), "u8"))
+            self.v_cache = wrap(DTensor.zeros((n_sets, Nkv, max_seq, D // 32 * nb), "u8"))
         elif kv_type == "f16":
             self.k_cache = DTensor.zeros((n_sets, Nkv, max_seq, D), "f16")
             self.v_cache = DTensor.zeros((n_sets, Nkv, max_seq, D), "f16")
         else:
-            raise ValueError("kv_type: q8_0 or f16")
+            raise ValueError("kv_type: q8_0, q4_0 or f16")
         self._bufs = {}
 
     def _buf(self, name, shape, dtype="f32"):
@@ -94,20 +109,17 @@ class Qwen3Layer:
         return b
 
     def _cache_view(self, c, s0, n, read_len):
-        if isinstance(c, ops.Q8):
-            return ops.Q8(c.data[s0:s0 + n, :, :read_len])
+        if isinstance(c, (ops.Q8, ops.Q4)):
+            return type(c)(c.data[s0:s0 + n, :, :read_len])
         return c[s0:s0 + n, :, :read_len]
 
-    def forward(self, hidden, pos, sets, s0: int, read_len: int, mask, out=None):
-        """hidden (N, H) F32 -> new hidden (N, H); pos, sets: (N,) I32 device tensors."""
+    def forward(self, hidden, pos, sets, s0: int, read_len: int, mask, out=None, adapter_ids=None):
+        """hidden (N, H) F32 -> new hidden (N, H); pos, sets: (N,) I32 device tensors, as
+        adapter_ids, each row's adapter (negative: none)."""
         N, Nh, Nkv, D = hidden.shape[0], self.Nh, self.Nkv, self.D
         st = self.stream
         qkv_dim = (Nh + 2 * Nkv) * D
-        # the input norm and the QKV product in one call: the normalized rows are
-        # made inside the quantization of the product's x
-        qkv = ops.mul_mat_q8_0_rms_norm(self.w["qkv"], hidden, self.in_norm_w, self.eps,
-                                        out=self._buf("qkv", (N, qkv_dim)), workspace=self._ws("qkv", hidden),
-                                        stream=st)
+        qkv = self._qkv(hidden, qkv_dim, adapter_ids)
         q = qkv[:, 0:Nh * D].unflatten(1, (Nh, D))
         k = qkv[:, Nh * D:(Nh + Nkv) * D].unflatten(1, (Nkv, D))
         v = qkv[:, (Nh + Nkv) * D:qkv_dim].unflatten(1, (Nkv, D))
@@ -122,27 +134,34 @@ class Qwen3Layer:
         attn = self._buf("attn", (N, 1, Nh, D))
         ws = self._fa_ws(qf, kv, vv)
         ops.flash_attn_ext(qf, kv, vv, mask, 1.0 / math.sqrt(D), out=attn, workspace=ws, stream=st)
-        return self._tail(hidden, attn.view(N, Nh * D), out)
+        return self._tail(hidden, attn.view(N, Nh * D), out, adapter_ids)
 
-    def prefill(self, hidden, kv_pos, s0: int, out=None):
+    def prefill(self, hidden, kv_pos, s0: int, out=None, adapter_ids=None):
         """hidden (N, S, H) F32 -> new hidden (N, S, H): S new tokens of each of N
         sequences; kv_pos (host ints, N): the slot of each sequence's first new
-        token (its earlier tokens already in the cache); sequence b uses set s0 + b.
-        prefill_inputs then prefill_run."""
-        inp = self.prefill_inputs(kv_pos, hidden.shape[1], s0)
+        token (its earlier tokens already in the cache); sequence b uses set s0 + b
+        and the adapter adapter_ids[b] (host ints, negative: none). prefill_inputs
+        then prefill_run."""
+        inp = self.prefill_inputs(kv_pos, hidden.shape[1], s0, adapter_ids)
         self._inputs = inp  # alive until the next call: the launches read them
         return self.prefill_run(hidden, inp, out)
 
-    def prefill_inputs(self, kv_pos, S: int, s0: int) -> dict:
+    def prefill_inputs(self, kv_pos, S: int, s0: int, adapter_ids=None) -> dict:
         """The host-built inputs of a prefill step, uploaded (qwen3-lm.h:513-533):
-        token positions, each sequence's first slot and set, the causal mask."""
+        token positions, each sequence's first slot and set, the causal mask, and
+        the tokens' adapters."""
         kv_pos = np.asarray(kv_pos, np.int64).reshape(-1)
         N = len(kv_pos)
-        max_seq = self.k_cache.data.shape[2] if isinstance(self.k_cache, ops.Q8) else self.k_cache.shape[2]
+        max_seq = (self.k_cache if self.kv_type == "f16" else self.k_cache.data).shape[2]
         kv_len = int((kv_pos + S).max())
         if kv_pos.min() < 0 or kv_len > max_seq:
             raise ValueError(f"prefill: slots [kv_pos, kv_pos + {S}) must lie in [0, {max_seq})")
-        return {"S": S, "s0": s0, "kv_len": kv_len,
+        if adapter_ids is not None:
+            ids = np.asarray(adapter_ids, np.int32).reshape(-1)
+            if len(ids) != N:
+                raise ValueError("prefill: one adapter id per sequence")
+            adapter_ids = DTensor.from_numpy(np.repeat(ids, S))
+        return {"S": S, "s0": s0, "kv_len": kv_len, "adapter_ids": adapter_ids,
                 "pos": DTensor.from_numpy((kv_pos[:, None] + np.arange(S)[None, :]).astype(np.int32).reshape(N * S)),
                 "pos0": DTensor.from_numpy(kv_pos.astype(np.int32)),
                 "sets": DTensor.from_numpy(np.arange(s0, s0 + N, dtype=np.int32)),
@@ -159,8 +178,7 @@ class Qwen3Layer:
         T = N * S
         h2 = hidden.view(T, H)
         qkv_dim = (Nh + 2 * Nkv) * D
-        qkv = ops.mul_mat_q8_0_rms_norm(self.w["qkv"], h2, self.in_norm_w, self.eps,
-                                        out=self._buf("qkv", (T, qkv_dim)), workspace=self._ws("qkv", h2), stream=st)
+        qkv = self._qkv(h2, qkv_dim, inp["adapter_ids"])
         q = qkv[:, 0:Nh * D].unflatten(1, (Nh, D))
         k = qkv[:, Nh * D:(Nh + Nkv) * D].unflatten(1, (Nkv, D))
         v = qkv[:, (Nh + Nkv) * D:qkv_dim].unflatten(1, (Nkv, D))
@@ -175,32 +193,66 @@ class Qwen3Layer:
         attn = self._buf("attn", (N, S, Nh, D))
         ws = self._fa_ws(qf, kv, vv)
         ops.flash_attn_ext(qf, kv, vv, mask, 1.0 / math.sqrt(D), out=attn, workspace=ws, stream=st)
-        y = self._tail(h2, attn.view(T, Nh * D), None if out is None else out.view(T, H))
+        y = self._tail(h2, attn.view(T, Nh * D), None if out is None else out.view(T, H), inp["adapter_ids"])
         return y.view(N, S, H)
 
-    def _tail(self, hidden, a2, out):
+    def _adapted(self, name, ids):
+        return ids is not None and name in self.adapters
+
+    def _lora(self, name, y, x, ids):
+        """The rows' low-rank updates of product `name`, added to y in place."""
+        if self._adapted(name, ids):
+            a, b = self.adapters[name]
+            ws = self._buf("ws_lora_" + name, (max(ops.lora_add_workspace(x, a, b), 16),), "u8")
+            ops.lora_add(y, x, a, b, ids, self.adapter_scales, out=y, workspace=ws, stream=self.stream)
+        return y
+
+    def _qkv(self, hidden, qkv_dim, ids):
+        """The input norm and the QKV product of rows of hidden."""
+        N, st = hidden.shape[0], self.stream
+        if self._adapted("qkv", ids):
+            n1 = ops.rms_norm(hidden, self.eps, w=self.in_norm_w, out=self._buf("n1", (N, self.H)), stream=st)
+            qkv = ops.mul_mat_q8_0(self.w["qkv"], n1, out=self._buf("qkv", (N, qkv_dim)),
+                                   workspace=self._ws("qkv", n1), stream=st)
+            return self._lora("qkv", qkv, n1, ids)
+        # the norm and the product in one call: the normalized rows are made inside
+        # the quantization of the product's x
+        return ops.mul_mat_q8_0_rms_norm(self.w["qkv"], hidden, self.in_norm_w, self.eps,
+                                         out=self._buf("qkv", (N, qkv_dim)), workspace=self._ws("qkv", hidden),
+                                         stream=st)
+
+    def _tail(self, hidden, a2, out, ids):
         """The O product, the residual sums, the post-attention norm and the MLP on
         rows of hidden (rows, H) and attention output a2 (rows, Nh * D)."""
         N, H, I = hidden.shape[0], self.H, self.I
         st = self.stream
         ao = ops.mul_mat_q8_0(self.w["o"], a2, out=self._buf("ao", (N, H)), workspace=self._ws("o", a2), stream=st)
-        if self.clamp_fp16:
-            h1, n2 = ops.add_rms_norm(hidden, ao, self.eps, w=self.post_norm_w, clamp=(-FP16_MAX, FP16_MAX),
+        self._lora("o", ao, a2, ids)
+        clamp = (-FP16_MAX, FP16_MAX) if self.clamp_fp16 else None
+        if self.clamp_fp16 or self._adapted("gu", ids):
+            h1, n2 = ops.add_rms_norm(hidden, ao, self.eps, w=self.post_norm_w, clamp=clamp,
                                       out_sum=self._buf("h1", (N, H)), out_norm=self._buf("n2", (N, H)), stream=st)
             gu = ops.mul_mat_q8_0(self.w["gu"], n2, out=self._buf("gu", (N, 2 * I)), workspace=self._ws("gu", n2),
                                   stream=st)
+            self._lora("gu", gu, n2, ids)
         else:
             # the residual add, the post-attention norm and the gate/up product in one call
             h1, gu = ops.mul_mat_q8_0_add_rms_norm(self.w["gu"], hidden, ao, self.post_norm_w, self.eps,
                                                    out_sum=self._buf("h1", (N, H)), out=self._buf("gu", (N, 2 * I)),
                                                    workspace=self._ws("gu", hidden), stream=st)
+        y = out if out is not None else self._buf("out", (N, H))
+        if self._adapted("down", ids):
+            ff = ops.swiglu(gu, out=self._buf("ff", (N, I)), stream=st)
+            dn = ops.mul_mat_q8_0(self.w["down"], ff, out=self._buf("dn", (N, H)), workspace=self._ws("down", ff),
+                                  stream=st)
+            self._lora("down", dn, ff, ids)
+            return (ops.add_clamp if self.clamp_fp16 else ops.add)(h1, dn, out=y, stream=st)
         # swiglu, the down projection and the residual add in one call: the SwiGLU
         # values are made inside the quantization of the product's x, and h1 is
         # added (then clamped under clamp_fp16) where the product's sum is formed
         # (bit-identical to the three ops)
-        y = out if out is not None else self._buf("out", (N, H))
-        return ops.mul_mat_q8_0_swiglu_add(self.w["down"], gu, h1, clamp=(-FP16_MAX, FP16_MAX) if self.clamp_fp16 else None,
-                                           out=y, workspace=self._ws_glu("down", gu), stream=st)
+        return ops.mul_mat_q8_0_swiglu_add(self.w["down"], gu, h1, clamp=clamp, out=y,
+                                           workspace=self._ws_glu("down", gu), stream=st)
 
     def _ws(self, name, x):
         need = ops.mul_mat_q8_0_workspace(self.w[name], x)
@@ -216,3 +268,24 @@ class Qwen3Layer:
 
 
 Qwen3DecodeLayer = Qwen3Layer  # the name the decode-only callers use
+
+
+class Qwen3Head:
+    def __init__(self, w_out, norm_w, V: int, eps: float = 1e-6, stream=None):
+        """w_out: the vocabulary's Q8 weights in the GGUF layout (repacked here once); norm_w: F32 DTensor."""
+        self.V, self.eps, self.stream, self.norm_w = V, eps, stream, norm_w
+        self.w = ops.q8_0_repack(w_out, stream=stream)
+        self._bufs = {}
+
+    _buf = Qwen3Layer._buf
+
+    def forward(self, hidden, out=None, **adjust):
+        """hidden (N, H) F32 -> logits (N, V): the final norm and the product in one call, then
+        ops.logits_adjust in place with the tensors given (history, lengths, penalties, bias,
+        allowed, state, err), none of them the bare logits."""
+        ws = self._buf("ws", (max(ops.mul_mat_q8_0_workspace(self.w, hidden), 1),), "u8")
+        y = out if out is not None else self._buf("logits", (hidden.shape[0], self.V))
+        ops.mul_mat_q8_0_rms_norm(self.w, hidden, self.norm_w, self.eps, out=y, workspace=ws, stream=self.stream)
+        if adjust:
+            ops.logits_adjust(y, out=y, stream=self.stream, **adjust)
+        return y
