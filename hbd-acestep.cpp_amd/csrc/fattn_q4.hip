@@ -19,6 +19,7 @@
 //         d above 8188 would leave fp16: tiles with one scale v by 2^-4, P by 2^4.
 // Sums, maxima and the running output are fp32.
 #include "launch.h"
+#include "rules.h"
 
 namespace mi {
 
@@ -152,6 +153,8 @@ __device__ __forceinline__ constexpr int fa4_slot(int e) {
     return (e & 2) * 2 + (e & 1) * 2 + (e >> 2);
 }
 
+typedef uint32_t fa4_u2h __attribute__((ext_vector_type(2), aligned(2)));  // 4 mask values
+
 // Query rows (query position, head) of a KV head in tiles of 16, keys split over
 // workgroups of W waves, a wave taking every (splits * W)-th tile of TK keys. With
 // v_mfma_f32_16x16x32_f16 (lane l: A[l%16][8(l/16)+e], B[8(l/16)+e][l%16],
@@ -201,8 +204,9 @@ __global__ void __launch_bounds__(64 * W) k_fa4_dec(const FaArgs a) {
     const int      c16 = lane & 15, q4 = lane >> 4;
     const uint32_t item  = blockIdx.x / (uint32_t) a.splits;
     const uint32_t split = blockIdx.x - item * (uint32_t) a.splits;
-    const uint32_t bg    = item / (uint32_t) a.rblocks;
-    const int      rt    = (int) (item - bg * (uint32_t) a.rblocks);
+    const uint32_t nbg   = (uint32_t) (a.nb * a.nkv);
+    const int      rt    = (int) (item / nbg);  // the row tiles of a KV head nbg workgroups apart: one XCD's L2 where 8 divides it
+    const uint32_t bg    = item - (uint32_t) rt * nbg;
     const uint32_t b     = bg / (uint32_t) a.nkv;
     const uint32_t g     = bg - b * (uint32_t) a.nkv;
     const int      row   = rt * 16 + c16 < a.rows ? rt * 16 + c16 : a.rows - 1;  // past the end: the last row again
@@ -264,7 +268,7 @@ __global__ void __launch_bounds__(64 * W) k_fa4_dec(const FaArgs a) {
     const int ntile = (a.n_kv + TK - 1) / TK;
     const int step  = a.splits * W;
     Fa4Raw    kr[IPL], vr[IPL];
-    uint16_t  mr[MS == 2 ? MT : 1][4];
+    fa4_u2h  mr[MS == 2 ? MT : 1];  // the lane's mask values, 4 keys each
     int       ko[IPL], vo[IPL];
 #pragma unroll
     for (int i = 0; i < IPL; ++i) {
@@ -286,10 +290,16 @@ __global__ void __launch_bounds__(64 * W) k_fa4_dec(const FaArgs a) {
         if constexpr (MS == 2) {
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int key = 16 * mt + 4 * q4 + r;
-                    mr[mt][r]     = *(const uint16_t *) (mrow + (int64_t) (t0 + (key < last ? key : last)) * 2);
+                const int key = t0 + 16 * mt + 4 * q4;
+                if (a.n_kv >= 4) {  // 4 keys in one load, the last ones from the row's end (shifted at their use)
+                    const char * mp = mrow + (int64_t) (key < a.n_kv - 4 ? key : a.n_kv - 4) * 2;
+                    mr[mt] = *(const fa4_u2h *) mp;
+                } else {
+                    for (int r = 0; r < 4; ++r) {
+                        const int      at = key + r < a.n_kv ? key + r : a.n_kv - 1;
+                        const uint32_t x  = *(const uint16_t *) (mrow + (int64_t) at * 2);
+                        mr[mt][r / 2]     = r & 1 ? mr[mt][r / 2] | x << 16 : x;
+                    }
                 }
             }
         }
@@ -342,10 +352,16 @@ __global__ void __launch_bounds__(64 * W) k_fa4_dec(const FaArgs a) {
             } else {
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) {
+                    uint64_t x = 0;
+                    if constexpr (MS == 2) {
+                        const int over = a.n_kv >= 4 ? t0 + 16 * mt + 4 * q4 + 4 - a.n_kv : 0;
+                        x              = (uint64_t) mr[mt].y << 32 | mr[mt].x;
+                        x              = over > 0 && over < 4 ? x >> (16 * over) : x;
+                    }
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const bool in = t0 + 16 * mt + 4 * q4 + r < a.n_kv;
-                        ms[mt][r]     = !in ? -INFINITY : MS == 2 ? f16_lo(mr[MS == 2 ? mt : 0][r]) * FA4_LOG2E : 0.0f;
+                        ms[mt][r]     = !in ? -INFINITY : MS == 2 ? f16_lo((uint32_t) (x >> (16 * r))) * FA4_LOG2E : 0.0f;
                         const uint64_t v = __builtin_amdgcn_ballot_w64(ms[mt][r] != -INFINITY);
 #pragma unroll
                         for (int gr = 0; gr < 4; ++gr) {
@@ -569,9 +585,9 @@ __global__ void __launch_bounds__(64 * W) k_fa4_dec(const FaArgs a) {
 // (m, l), before the weights are known: one round of memory latency for up to SG * PRE splits.
 constexpr int FA4_MAX_SPLITS = 1024;
 
-template <int D>
+template <int D, int PRE>
 __global__ void __launch_bounds__(256) k_fa4_combine(const FaArgs a) {
-    constexpr int C4 = D / 4, SG = 256 / C4, PRE = 8;
+    constexpr int C4 = D / 4, SG = 256 / C4;
     __shared__ float                wsh[FA4_MAX_SPLITS];
     __shared__ float                red[8];
     __shared__ __align__(16) fa4_f4 part[SG][C4];
@@ -657,6 +673,57 @@ __global__ void __launch_bounds__(256) k_fa4_combine(const FaArgs a) {
         } else {
             *(fa4_u2u *) (yp + 8 * tid) = fa4_u2u{ pack_bf16x2(t[0], t[1]), pack_bf16x2(t[2], t[3]) };
         }
+    }
+}
+
+// The same for up to S splits: D / 4 lanes per row, a lane's columns of every split in registers,
+// no exchange between lanes.
+template <int D, int S>
+__global__ void __launch_bounds__(256) k_fa4_combine_few(const FaArgs a) {
+    constexpr int  C4   = D / 4, RW = 256 / C4;
+    const int      c    = threadIdx.x % C4;
+    const uint32_t nrec = (uint32_t) (a.nb * a.nkv) * (uint32_t) a.rows;
+    const uint32_t rec  = blockIdx.x * RW + threadIdx.x / C4;
+    if (rec >= nrec) {
+        return;
+    }
+    const int     last = a.splits - 1;
+    const float * p    = a.ws + (int64_t) rec * a.splits * (D + 4);
+    fa4_f4        pv[S];
+    float         m[S], l[S];
+#pragma unroll
+    for (int s = 0; s < S; ++s) {  // past the last split: the last one again, weight 0
+        const float * ps = p + (int64_t) (s < last ? s : last) * (D + 4);
+        m[s]             = ps[0];
+        l[s]             = ps[1];
+        pv[s]            = *(const fa4_f4 *) (ps + 4 + 4 * c);
+    }
+    const uint32_t bg  = rec / (uint32_t) a.rows;
+    const int      row = (int) (rec - bg * (uint32_t) a.rows);
+    const uint32_t b   = bg / (uint32_t) a.nkv;
+    const uint32_t g   = bg - b * (uint32_t) a.nkv;
+    const int      iq = row / a.rk, h = (int) g * a.rk + (row - iq * a.rk);
+    float          mm = m[0], lt = 0.0f;
+#pragma unroll
+    for (int s = 1; s < S; ++s) {
+        mm = fmaxf(mm, m[s]);
+    }
+    fa4_f4 t = { 0.0f, 0.0f, 0.0f, 0.0f };
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+        const float w = s > last || m[s] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[s] - mm);
+        lt            = w == 0.0f ? lt : __builtin_fmaf(w, l[s], lt);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            t[e] = w == 0.0f ? t[e] : __builtin_fmaf(w, pv[s][e], t[e]);
+        }
+    }
+    t *= 1.0f / lt;  // no live key: 0 * inf
+    char * yp = a.y + (int64_t) b * a.y3 + (int64_t) iq * a.y2 + (int64_t) h * a.y1;
+    if (a.ty == MI_TYPE_F32) {
+        *(fa4_f4u *) (yp + 16 * c) = t;
+    } else {
+        *(fa4_u2u *) (yp + 8 * c) = fa4_u2u{ pack_bf16x2(t[0], t[1]), pack_bf16x2(t[2], t[3]) };
     }
 }
 
@@ -996,7 +1063,7 @@ k_fa4_pre(const FaArgs a) {
                         kx[mt][blk] = *(const fa4_h8 *) (kl + (32 * kk + 16 * mt + c16) * F::KS + q4 * 16 + blk * 64);
                     }
                 }
-                // mask values of the lane's scores in units of log2, 4 keys a load where rows are 8-byte aligned
+                // mask values of the lane's scores in units of log2, 4 keys a load (rows lie at any 2 bytes)
                 fa4_f4 mk[RT][2];
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) {
@@ -1008,8 +1075,8 @@ k_fa4_pre(const FaArgs a) {
                         uint32_t x[2][2] = {};
                         if constexpr (MSK) {
                             const char * mp = mrow[rt] + (int64_t) (t0 + 32 * kk + 4 * q4) * 2;
-                            if (a.mvec && t0 + T <= a.n_kv) {
-                                const uint2 y = *(const uint2 *) mp, z = *(const uint2 *) (mp + 32);
+                            if (t0 + T <= a.n_kv) {
+                                const fa4_u2h y = *(const fa4_u2h *) mp, z = *(const fa4_u2h *) (mp + 32);
                                 x[0][0] = y.x;
                                 x[0][1] = y.y;
                                 x[1][0] = z.x;
@@ -1189,7 +1256,6 @@ k_fa4_pre(const FaArgs a) {
 }
 
 constexpr int FA4_W        = 4;   // waves per workgroup of the kernel for few rows
-constexpr int FA4_DEC_ROWS = 32;  // rows (query position, head) of a KV head that it takes
 
 // rows of a workgroup of the kernel for many rows
 static int fa4_bq(int D, bool f32) {
@@ -1215,32 +1281,20 @@ void flash_attn_q4_plan(FaArgs & a, int D) {
         a.splits = 0;  // keys are counted in 32 bits, 8 tiles of every wave ahead; a tile's offsets too
         return;
     }
-    a.mfma = a.rows > FA4_DEC_ROWS && a.ngq <= 65535 && (int64_t) a.nb * a.nh <= 65535;
-    int64_t       items, want, most, least = 1;
-    const int     tk    = a.mfma ? (D == 256 ? 32 : 64) : (D == 64 ? 64 : 32);  // keys per tile
-    const int64_t tiles = ((int64_t) a.n_kv + tk - 1) / tk;
-    if (a.mfma) {
-        // the workspace is sized without y: its type (rows per workgroup) must not change the splits
-        a.rblocks = (a.rows + 127) / 128;
-        items     = (int64_t) a.nb * a.nkv * a.rblocks;
-        want      = (int64_t) num_cus() * 2 / items;
-        most      = (tiles + 7) / 8;
-        least     = (tiles + FA4_PRE_TILES - 1) / FA4_PRE_TILES;
-    } else {
-        items = (int64_t) a.nb * a.nkv * a.rblocks;
-        want = (int64_t) num_cus() * (D == 256 ? 1 : 3) / items;
-        most = (tiles + 2 * FA4_W - 1) / (2 * FA4_W);
-    }
-    most     = most < FA4_MAX_SPLITS ? most : FA4_MAX_SPLITS;
-    want     = want < most ? want : most;
-    a.splits = (int) (want < least ? least : want);
-    if (a.splits > FA4_MAX_SPLITS || items * a.splits >= ((int64_t) 1 << 31)) {
-        a.splits = 0;  // more than the merge or a grid takes
-        return;
-    }
+    const Fa4Plan p     = fa4_plan((int64_t) a.nb * a.nkv, a.rows, a.n_kv, D, a.ty == MI_TYPE_F32, a.n_q == 1, num_cus());
+    a.mfma              = p.many && a.ngq <= 65535 && (int64_t) a.nb * a.nh <= 65535;
+    const int64_t tiles = ((int64_t) a.n_kv + 63) / 64 * (D == 256 ? 2 : 1);
+    const int64_t least = a.mfma ? (tiles + FA4_PRE_TILES - 1) / FA4_PRE_TILES : 1;
     if (a.mfma) {
         const int bq = fa4_bq(D, a.ty == MI_TYPE_F32);
         a.rblocks    = (a.rows + bq - 1) / bq;
+    }
+    const int64_t items = (int64_t) a.nb * a.nkv * a.rblocks;
+    int64_t       want  = p.many == (a.mfma != 0) ? p.splits : 1;
+    want                = want < FA4_MAX_SPLITS ? want : FA4_MAX_SPLITS;
+    a.splits = (int) (want < least ? least : want);
+    if (a.splits > FA4_MAX_SPLITS || items * a.splits >= ((int64_t) 1 << 31)) {
+        a.splits = 0;  // more than the merge or a grid takes
     }
 }
 
@@ -1251,7 +1305,15 @@ static size_t fa4_parts(const FaArgs & a, int D) {
 }
 
 size_t flash_attn_q4_workspace(const FaArgs & a, int D) {
-    return fa4_parts(a, D) + (a.mfma ? (size_t) a.nb * a.nh * a.ngq * ((a.n_kv + 63) / 64) : 0);
+    size_t need = 0;
+    for (const int ty : { MI_TYPE_F32, MI_TYPE_BF16 }) {  // whatever y is: a caller asks before there is one
+        FaArgs t = a;
+        t.ty     = ty;
+        flash_attn_q4_plan(t, D);
+        const size_t n = fa4_parts(t, D) + (t.mfma ? (size_t) t.nb * t.nh * t.ngq * ((t.n_kv + 63) / 64) : 0);
+        need           = n > need ? n : need;
+    }
+    return need;
 }
 
 template <int D, bool OS>
@@ -1275,7 +1337,19 @@ static void launch_dec(const FaArgs & a, hipStream_t s) {
         MI_LAUNCH((k_fa4_dec<D, OS, 2, FA4_W>), grid, wg, 0, s, a);
     }
     if (a.splits > 1) {
-        MI_LAUNCH((k_fa4_combine<D>), dim3((uint32_t) (a.nb * a.nkv * a.rows)), dim3(256), 0, s, a);
+        const dim3 grid_c((uint32_t) ((int64_t) a.nb * a.nkv * a.rows));
+        const dim3 grid_f((uint32_t) (((int64_t) a.nb * a.nkv * a.rows + 1024 / D - 1) / (1024 / D)));
+        if (a.splits <= 2) {
+            MI_LAUNCH((k_fa4_combine_few<D, 2>), grid_f, dim3(256), 0, s, a);
+        } else if (a.splits <= 4) {
+            MI_LAUNCH((k_fa4_combine_few<D, 4>), grid_f, dim3(256), 0, s, a);
+        } else if (a.splits <= 8) {
+            MI_LAUNCH((k_fa4_combine_few<D, 8>), grid_f, dim3(256), 0, s, a);
+        } else if (a.splits <= 2 * 1024 / D) {
+            MI_LAUNCH((k_fa4_combine<D, 2>), grid_c, dim3(256), 0, s, a);
+        } else {
+            MI_LAUNCH((k_fa4_combine<D, 8>), grid_c, dim3(256), 0, s, a);
+        }
     }
 }
 

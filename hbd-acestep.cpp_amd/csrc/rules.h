@@ -77,4 +77,57 @@ inline bool logits_small_tiles(uint32_t rows, int64_t n_vocab, uint32_t cus) {
     return (int64_t) rows * ((n_vocab + 8191) / 8192) < 4 * (int64_t) cus;
 }
 
+// Attention over Q4_0 K and V: the keys of a row are split over `s` workgroups where that saves
+// more than it costs. A split saves tile_ns of every tile of the row's keys that is left to another
+// workgroup, and costs a launch that joins the results (2300 ns) and the traffic of a partial
+// result, row_ps picoseconds per row and split; `want` workgroups per row are resident at once.
+// us, 128 values, 16 heads on 8, unsplit / split in 2 / 3 / 4 / 6: one row per head of 256 keys 10.4 /
+// 12.0, of 512 13.5 / - / 11.9; 64 positions on 2064 keys 44.7 / 29.4 / 23.8 / 21.6 / 22.8; 512 on
+// 512 23.5 / 34.4; many rows a workgroup: 1024 on 5120 418 / 224 / 162 / 139 / 174
+inline int64_t fa4_splits(int64_t tiles, int64_t rows, int64_t want, int64_t tile_ns, int64_t row_ps) {
+    int64_t s = 1;
+    while (s < want && (s + 1) * (s + 1) * row_ps * rows <= tiles * tile_ns * 1000) {
+        ++s;
+    }
+    return tiles * tile_ns * (s - 1) / s < 2300 + row_ps * rows * s / 1000 ? 1 : s;
+}
+
+struct Fa4Plan {
+    bool    many;    // workgroups of many rows (k_fa4_pre), not of 16 (k_fa4_dec)
+    int64_t splits;  // of a row's keys
+};
+
+// Which of the two kernels takes `rows` rows of each of `heads` KV heads (times sequences) on n_kv
+// keys of d values, one: a single query position. The kernel for 16 rows per workgroup has the
+// shorter way from the first key to the last (four waves share a tile's turn), the one for many
+// rows unpacks a key once for 128 or 256 of them. Their times in ns as the sums of what was
+// measured one by one; both sides, us, 16 rows / many, the kernel's best splits (F32 y, BF16 y):
+//   16 heads on 8: 64 positions on 464 keys 13.3 / 22.8, 12.5 / 18.8; 257 on 387 18.9 / 35.8, 16.8 / 24.2;
+//                  512 on 512 23.5 / 34.8, 20.9 / 26.3; 1024 on 1024 65 / 51, 52 / 37; 2048 on 2048 207 / 98, 146 / 58
+//   32 on 8, 8 sequences: 16 on 4016 59 / 96, 48 / 40; 64 on 4064 194 / 108, 146 / 66; 128 on 128 45 / 28, 35 / 17
+inline Fa4Plan fa4_plan(int64_t heads, int64_t rows, int64_t n_kv, int d, bool f32, bool one, int64_t cus) {
+    const int64_t all = heads * rows;
+    // 16 rows a workgroup
+    const int64_t tk = d == 64 ? 64 : 32, tiles = (n_kv + tk - 1) / tk, items = heads * ((rows + 15) / 16);
+    const int64_t way = (one ? 1100 : 2200) / 4;  // a tile, one of four waves
+    const int64_t most = (tiles + 7) / 8;         // two tiles a wave
+    int64_t       want = (d == 256 ? 1 : 3) * cus / items;
+    Fa4Plan       p{ false, fa4_splits(tiles, all, want < most ? want : most, way, 800) };
+    if (rows <= 32) {
+        return p;
+    }
+    const int64_t work = (f32 ? 12 : 9) * items * p.splits + (f32 ? 142 : 108) * (d == 256 ? 2 : 1) * items * tiles / 100;
+    const int64_t last = tiles * way / p.splits;
+    const int64_t few  = 8500 + (work > last ? work : last) + (p.splits > 1 ? 2300 + all * p.splits * 8 / 10 : 0);
+    // many
+    const int64_t bq = f32 && d == 128 ? 256 : 128, tkm = d == 256 ? 32 : 64, tm = (n_kv + tkm - 1) / tkm;
+    const int64_t wgs = heads * ((rows + bq - 1) / bq), slots = cus * (d == 256 || (f32 && d == 128) ? 1 : 2);
+    const int64_t ns  = f32 ? (d == 128 ? 5100 : 2600) : (d == 64 ? 1000 : 2000);  // a tile
+    const int64_t fit = (tm + 1) / 2;  // two tiles a workgroup
+    want              = slots / wgs;
+    const int64_t s   = fa4_splits(tm, all, want < fit ? want : fit, ns, 250);
+    const int64_t many = 14000 + tm * ns / s * ((wgs * s + slots - 1) / slots) + (s > 1 ? 2300 + all * s / 4 : 0);
+    return many < few ? Fa4Plan{ true, s } : p;
+}
+
 }  // namespace mi
