@@ -166,7 +166,9 @@ __global__ void __launch_bounds__(256) k_lora_down(const LoraArgs a) {
 // y = y0 + B (scale h). A workgroup: 16 TT rows of x (blockIdx.x) and every gridDim.y-th block of
 // 64 NT columns of y, a wave 16 NT of them. h is summed over the key shares, scaled and split
 // once, into LDS; a block's y0 is loaded under the block before it. RS: steps of 32 ranks; U:
-// adapters whose weights are loaded before the first is multiplied.
+// adapters whose weights are loaded before the first is multiplied. With NT 1 (few rows) the distinct
+// adapters of the tile are shared out over gridDim.z workgroups, each storing the rows of its own
+// (and the first those without one): a row has one adapter, so there is nothing to sum.
 // Column c of product i is column NT c + i of the wave's: a lane holds NT consecutive columns of
 // 4 rows, and with NT 4 a load or store of y covers 256 consecutive bytes of a row (products of
 // 16 consecutive columns each: 64, and 167 us instead of 138 for 4005 x 19456 at rank 32).
@@ -181,7 +183,21 @@ __global__ void __launch_bounds__(256) k_lora_up(const LoraArgs a) {
     const int      wv   = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t t0   = blockIdx.x * R;
     const int32_t  idl  = lr_id(a, t0 + (lane < R ? lane : R));  // lanes 0 .. R - 1: the rows' adapters
-    const uint64_t rows = __builtin_amdgcn_ballot_w64(idl >= 0 && lane < R);
+    uint64_t       rows = __builtin_amdgcn_ballot_w64(idl >= 0 && lane < R), own = ~0ull;  // with an adapter; to be stored
+    if constexpr (NT == 1) {
+        own = blockIdx.z == 0 ? ~rows : 0;
+        uint64_t left = rows;
+        for (uint32_t j = 0; left; j = j + 1 < gridDim.z ? j + 1 : 0) {
+            const uint64_t mine = __builtin_amdgcn_ballot_w64(idl == __builtin_amdgcn_readlane(idl, __builtin_ctzll(left)));
+            left &= ~mine;
+            own |= j == blockIdx.z ? mine : 0;
+        }
+        own &= t0 + R <= a.m ? (1ull << R) - 1 : (1ull << (a.m - t0)) - 1;
+        rows &= own;
+        if (own == 0) {
+            return;  // the whole workgroup
+        }
+    }
     int32_t        id[TT][4];
 #pragma unroll
     for (int tt = 0; tt < TT; ++tt) {
@@ -212,13 +228,13 @@ __global__ void __launch_bounds__(256) k_lora_up(const LoraArgs a) {
     for (int i = threadIdx.x; i < R * RS * 32; i += 256) {
         const int      t = i / (RS * 32), r = i - t * RS * 32;
         const int32_t  it  = __shfl(idl, t, 64);
-        const bool     on  = it >= 0 && r < (int) a.r;
+        const bool     on  = it >= 0 && r < (int) a.r && (NT != 1 || own >> t & 1);
         const uint32_t tr  = t0 + t < a.m ? t0 + t : a.m - 1;
         const float *  hp  = a.h + (int64_t) tr * a.rp + (r < (int) a.r ? r : 0);
         const int64_t  st  = (int64_t) a.m * a.rp;
         const float    sc  = a.scales && on ? *(const float *) (a.scales + (int64_t) it * a.s0) : 1.0f;
         float          v   = 0.0f;
-        for (uint32_t s = 0; s < a.ks; s += 16) {  // 16 shares in flight; rows without an adapter hold anything
+        for (uint32_t s = 0; on && s < a.ks; s += 16) {  // 16 shares in flight
             float p[16];
 #pragma unroll
             for (int q = 0; q < 16; ++q) {
@@ -328,7 +344,7 @@ __global__ void __launch_bounds__(256) k_lora_up(const LoraArgs a) {
             for (int tt = 0; tt < TT; ++tt) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    if (t0 + tt * 16 + 4 * q4 + e < a.m) {
+                    if (NT == 1 ? own >> (4 * q4 + e) & 1 : t0 + tt * 16 + 4 * q4 + e < a.m) {
                         *(lr_y *) (a.y + row(tt, e) * a.y1 + (int64_t) n * 4) = acc[tt][e];
                     }
                 }
@@ -397,7 +413,13 @@ template <int WT, int RS> static void launch_up(const LoraArgs & a, hipStream_t 
         const uint32_t want  = ((uint32_t) num_cus() * 8 + tiles - 1) / tiles;
         MI_LAUNCH((k_lora_up<WT, 4, TT, RS, 1>), dim3(tiles, want < blocks ? want : blocks), dim3(256), 0, s, a);
     } else {
-        MI_LAUNCH((k_lora_up<WT, 1, 1, RS, RS < 4 ? 4 : RS < 8 ? 2 : 1>), dim3((a.m + 15) / 16, (a.n + 63) / 64),
+        // the adapters of a tile over enough workgroups for 2 per CU (48 rows of 24 adapters, 2560
+        // columns at rank 64, both launches: 1 workgroup 20.4 us, for 1 per CU 17.4, 2 16.9, 4 18.7, 8 19.7)
+        const uint32_t wgs = (a.m + 15) / 16 * ((a.n + 63) / 64), most = a.n_ad < 16 ? (uint32_t) a.n_ad : 16;
+        uint32_t       z   = ((uint32_t) num_cus() * 2 + wgs - 1) / wgs;
+        z                  = z < most ? z : most;
+        z                  = z < a.m ? z : a.m;
+        MI_LAUNCH((k_lora_up<WT, 1, 1, RS, RS < 4 ? 4 : RS < 8 ? 2 : 1>), dim3((a.m + 15) / 16, (a.n + 63) / 64, z > 1 ? z : 1),
                   dim3(256), 0, s, a);
     }
 }
