@@ -1375,7 +1375,7 @@ static int lora_desc(const mi_tensor * x, const mi_tensor * a, const mi_tensor *
         return MI_ERR_SHAPE;
     }
     const int64_t m = nrows(*x), n = b->ne[1];
-    if (r > 256 || (m + 15) / 16 * ((n + 63) / 64) >= kMaxRows || (n + 63) / 64 > 65535) {
+    if (r > 256 || m > (1 << 30) || (m + 15) / 16 * ((n + 63) / 64) >= kMaxRows || (n + 63) / 64 > 65535) {
         return MI_ERR_UNSUPPORTED;
     }
     l      = LoraArgs{};
@@ -1538,8 +1538,8 @@ int mi_logits_adjust(const mi_tensor * logits, const mi_tensor * history, const 
     if (!aligned(d_err, 4)) {
         return MI_ERR_ALIGN;
     }
-    if (rows > 65535) {
-        return MI_ERR_UNSUPPORTED;  // a grid's second dimension
+    if (rows > 65535 || V > (1 << 30) || a.n_hist > (1 << 30)) {
+        return MI_ERR_UNSUPPORTED;  // a grid's second dimension; tokens and places are 32-bit
     }
     if (V == 0 || rows == 0) {
         return MI_OK;

@@ -1293,7 +1293,7 @@ void flash_attn_q4_plan(FaArgs & a, int D) {
     int64_t       want  = p.many == (a.mfma != 0) ? p.splits : 1;
     want                = want < FA4_MAX_SPLITS ? want : FA4_MAX_SPLITS;
     a.splits = (int) (want < least ? least : want);
-    if (a.splits > FA4_MAX_SPLITS || items * a.splits >= ((int64_t) 1 << 31)) {
+    if (a.splits > FA4_MAX_SPLITS || items * a.splits >= ((int64_t) 1 << 31) || (int64_t) a.nb * a.nkv * a.rows >= ((int64_t) 1 << 31)) {
         a.splits = 0;  // more than the merge or a grid takes
     }
 }

@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(256) k_logits(const LogitsArgs a) {
         const int32_t * hp  = (const int32_t *) (a.hist + (int64_t) row * a.h1);
         uint32_t        bad = 0;
         auto            put = [&](int32_t t) {
-            const uint32_t d = (uint32_t) (t - (int32_t) v0);  // both below 2^31: a token before the tile wraps past it
+            const uint32_t d = (uint32_t) t - (uint32_t) v0;  // a token before the tile, or negative, wraps past it
             if (d < (uint32_t) nv) {
                 atomicAdd(count + d, 1u);
             }

@@ -288,11 +288,12 @@ typedef uint32_t q4_u2 __attribute__((ext_vector_type(2), aligned(2)));  // 8 by
 
 // Q4_0 destinations: a wave takes 32 consecutive blocks, a lane pair a block, the first lane its
 // elements 0-15 and the second 16-31. Byte j holds the levels of elements j and j + 16, so the
-// lanes exchange their levels (one DPP swap) and store 8 of the 16 bytes each. What bounds it is
-// the arithmetic of the levels and addresses: with a sequence's tokens a multiple of the rows of a
-// wave, head and sequence are the wave's and their part of the addresses is scalar, and the source
-// is read without a detour through LDS (8 x 2048 tokens, 8 heads x 128, bf16, K and V: 20.3 us, 4.2 TB/s;
-// 21.7 with every lane finding its row three times, twice of them for lane-contiguous loads).
+// lanes exchange their levels (one DPP swap) and store 8 of the 16 bytes each. With a sequence's
+// tokens a multiple of the rows of a wave, head and sequence are the wave's and their part of the
+// addresses is scalar; the source is read without a detour through LDS. Memory bounds it: 8 x 2048
+// tokens of 8 heads x 128 in bf16, K and V, 20.3 us, 4.2 TB/s, where a read of a large buffer alone
+// reaches 4.0 and a copy 4.8 (21.7 us with every lane finding its row three times, two of them for
+// lane-contiguous loads into LDS).
 template <int TI>
 __global__ void __launch_bounds__(256) k_row_q4(const RowCopy K, const RowCopy V, uint32_t nbk, uint32_t nbv,
                                                 uint32_t wg_k, uint32_t nbpr, FastDiv dnbpr) {

@@ -261,7 +261,12 @@ int mi_timestep_embedding(const mi_tensor * t, int dim, int max_period, const mi
  * (query, head) rows per KV head, D = 128) reads the K/V rows of keys masked
  * for only some rows of a 64-key tile and multiplies them by 0, so F16/BF16
  * rows there must be finite (the reference clears its caches at allocation);
- * a Q8_0 V block with a non-finite scale counts as 0.
+ * a Q8_0 V block with a non-finite scale counts as 0. Over Q4_0 K and V a key that
+ * none of the rows a workgroup shares attends to (16 to 256 rows of a KV head; all of
+ * one position's with n_q = 1) counts as zeros whatever its bytes are; a block with a
+ * non-finite scale of a key that one of them attends to may make the others NaN as
+ * well. Q4_0 takes n_kv up to 2^27 and key strides below 32 MiB, others return
+ * MI_ERR_UNSUPPORTED. With BF16 y many rows of q read K rounded to fp16 (2^-11).
  * workspace: device memory of at least mi_flash_attn_ext_workspace() bytes
  * (for the partial results of a split key range; NULL when that is 0). The
  * size depends on the shapes and on the current device's CU count. */
@@ -399,6 +404,7 @@ int mi_mul_mat_q8_0_adaln(const void * w, int64_t k, int64_t n, const mi_tensor 
  *   ids:   I32 [m]; a negative id is a row without an adapter, y = y0; an id past the
  *          last adapter is taken as one and counted in *d_err when d_err != NULL
  *   scales: F32 [n_adapters] or NULL (1)
+ * Rows of A and B may lie at any element; m up to 2^30.
  * Products and sums keep fp32 accuracy (x and A x as three bf16 parts each on the
  * matrix cores). workspace: device memory of at least mi_lora_add_workspace() bytes,
  * 16-byte aligned; calls that share one race. The size depends on the shapes and on
@@ -426,7 +432,8 @@ int mi_lora_add(const mi_tensor * y0, const mi_tensor * x, const mi_tensor * a, 
  *              a state of the grammar allows token v; state: I32 [rows], each row's state
  *              (negative: no grammar; past the last: none, and counted in *d_err), or NULL
  *              (n_states 1: the same for all rows; n_states = rows: row r's own)
- * A row whose state allows nothing is all -inf. */
+ * A row whose state allows nothing is all -inf. Up to 65535 rows, 2^30 tokens and 2^30
+ * places of history (MI_ERR_UNSUPPORTED). */
 int mi_logits_adjust(const mi_tensor * logits, const mi_tensor * history, const mi_tensor * lengths,
                      const mi_tensor * penalties, const mi_tensor * bias, const mi_tensor * allowed,
                      const mi_tensor * state, const mi_tensor * y, int32_t * d_err, mi_stream stream);

@@ -85,3 +85,17 @@ def test_logits_adjust():
     big = [_t([V, 70000], data=d << 30) for d in (1, 2)]
     assert L.mi_logits_adjust(R(big[0]), None, None, None, None, None, None, R(big[1]), None, None) == -7
     assert L.mi_logits_adjust(R(_t([0, m])), None, None, None, None, None, None, R(_t([0, m])), None, None) == 0
+
+
+def test_sizes_past_32_bits():
+    """Rows, tokens and places that the kernels' 32-bit counters could not hold (views of one row at stride 0)."""
+    big = 1 << 31
+    x = _t([64, big - 1], nb=[4, 0, 0, 0])
+    ws = ctypes.c_size_t(0)
+    assert L.mi_lora_add_workspace(R(x), R(_t([64, 8, 1], BF16)), R(_t([8, 32, 1], BF16)), ctypes.byref(ws)) == -7
+    one = _t([1 << 30 | 32, 1], BF16)
+    assert L.mi_logits_adjust(R(one), None, None, None, None, None, None, R(one), None, None) == -7
+    lg, pen = _t([64, 2]), _t([3, 2])
+    for n in (1 << 30 | 1, big - 1):
+        assert L.mi_logits_adjust(R(lg), R(_t([n, 2], I32)), None, R(pen), None, None, None, R(lg), None, None) == -7
+    assert L.mi_logits_adjust(R(_t([8, 65536])), None, None, None, None, None, None, R(_t([8, 65536])), None, None) == -7
