@@ -835,12 +835,12 @@ k_fa4_pre(const FaArgs a) {
         }
     }
 
-    float  m[RT], l[RT];
-    fa4_f4 o[RT][2 * NB];
+    float  m[RT];
+    fa4_f4 o[RT][2 * NB], l[RT];  // l: the sum of p, in all 4 (A = ones)
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         m[rt] = -INFINITY;
-        l[rt] = 0.0f;
+        l[rt] = fa4_f4{ 0.0f, 0.0f, 0.0f, 0.0f };
 #pragma unroll
         for (int i = 0; i < 2 * NB; ++i) {
             o[rt][i] = fa4_f4{ 0.0f, 0.0f, 0.0f, 0.0f };
@@ -1049,7 +1049,8 @@ k_fa4_pre(const FaArgs a) {
                     raw[i] = load(i, t2, t2 < tend);
                 }
             }
-            const float pinv = fl & 1 ? 0.0625f : 1.0f;  // P is held 16 times as large where V is held / 16
+            const uint32_t one = fl & 1 ? 0x2c002c00u : 0x3c003c00u;  // 1/16 where V is held / 16 and P 16 times as large
+            const fa4_h8   ones = __builtin_bit_cast(fa4_h8, make_uint4(one, one, one, one));
             const float poff = fl & 1 ? FA4_OFF + 4.0f : FA4_OFF;
             // 32 keys at a time: few enough scores and operands that the LDS reads of both products can be
             // in flight before the first is used
@@ -1063,39 +1064,26 @@ k_fa4_pre(const FaArgs a) {
                         kx[mt][blk] = *(const fa4_h8 *) (kl + (32 * kk + 16 * mt + c16) * F::KS + q4 * 16 + blk * 64);
                     }
                 }
-                // mask values of the lane's scores in units of log2, 4 keys a load (rows lie at any 2 bytes)
-                fa4_f4 mk[RT][2];
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
-                    mk[rt][0] = mk[rt][1] = fa4_f4{ 0.0f, 0.0f, 0.0f, 0.0f };
-                }
-                if (!clean) {
+                // the mask of the lane's scores, 4 keys a load (rows lie at any 2 bytes)
+                uint32_t mx[RT][2][2] = {};
+                if (MSK && !clean) {
 #pragma unroll
                     for (int rt = 0; rt < RT; ++rt) {
-                        uint32_t x[2][2] = {};
-                        if constexpr (MSK) {
-                            const char * mp = mrow[rt] + (int64_t) (t0 + 32 * kk + 4 * q4) * 2;
-                            if (t0 + T <= a.n_kv) {
-                                const fa4_u2h y = *(const fa4_u2h *) mp, z = *(const fa4_u2h *) (mp + 32);
-                                x[0][0] = y.x;
-                                x[0][1] = y.y;
-                                x[1][0] = z.x;
-                                x[1][1] = z.y;
-                            } else {
+                        const char * mp = mrow[rt] + (int64_t) (t0 + 32 * kk + 4 * q4) * 2;
+                        if (t0 + T <= a.n_kv) {
+                            const fa4_u2h y = *(const fa4_u2h *) mp, z = *(const fa4_u2h *) (mp + 32);
+                            mx[rt][0][0] = y.x;
+                            mx[rt][0][1] = y.y;
+                            mx[rt][1][0] = z.x;
+                            mx[rt][1][1] = z.y;
+                        } else {
 #pragma unroll
-                                for (int e = 0; e < 8; ++e) {
-                                    const int      key = t0 + 32 * kk + 16 * (e / 4) + 4 * q4 + e % 4;
-                                    const int      at  = key < a.n_kv ? key : a.n_kv - 1;
-                                    const uint32_t y   = *(const uint16_t *) (mrow[rt] + (int64_t) at * 2);
-                                    x[e / 4][e % 4 / 2] |= y << (16 * (e % 2));
-                                }
+                            for (int e = 0; e < 8; ++e) {
+                                const int      key = t0 + 32 * kk + 16 * (e / 4) + 4 * q4 + e % 4;
+                                const int      at  = key < a.n_kv ? key : a.n_kv - 1;
+                                const uint32_t y   = *(const uint16_t *) (mrow[rt] + (int64_t) at * 2);
+                                mx[rt][e / 4][e % 4 / 2] |= y << (16 * (e % 2));
                             }
-                        }
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            const bool  in = t0 + 32 * kk + 16 * (e / 4) + 4 * q4 + e % 4 < a.n_kv;
-                            const float y  = (e & 1 ? f16_hi(x[e / 4][e % 4 / 2]) : f16_lo(x[e / 4][e % 4 / 2])) * FA4_LOG2E;
-                            mk[rt][e / 4][e % 4] = in ? y : -INFINITY;
                         }
                     }
                 }
@@ -1135,19 +1123,32 @@ k_fa4_pre(const FaArgs a) {
                     stage(kk, raw[kk], bf ^ 1, fn, live);  // past the last tile: zeros
                     raw[kk] = load(kk, t2, t2 < tend);
                 }
-                float lm[RT];
+                // scores in units of log2: s * fac
+                float fac[RT], lm[RT];
                 bool  grow = false;
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) {
-                    const float fac = qs[rt] * kf;
+                    fac[rt] = qs[rt] * kf;
+                }
+                if (!clean) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        s[rt][e / 4][e % 4] = __builtin_fmaf(s[rt][e / 4][e % 4], fac, mk[rt][e / 4][e % 4]);
+                    for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const bool     in = t0 + 32 * kk + 16 * (e / 4) + 4 * q4 + e % 4 < a.n_kv;
+                            const uint32_t w  = mx[rt][e / 4][e % 4 / 2];
+                            const float    y  = in ? (e & 1 ? f16_hi(w) : f16_lo(w)) * FA4_LOG2E : -INFINITY;
+                            s[rt][e / 4][e % 4] = __builtin_fmaf(s[rt][e / 4][e % 4], fac[rt], y);
+                        }
+                        fac[rt] = 1.0f;
                     }
+                }
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
                     float x = fmaxf(fmaxf(s[rt][0][0], s[rt][0][1]), s[rt][0][2]);
                     x       = fmaxf(fmaxf(x, s[rt][0][3]), s[rt][1][0]);
                     x       = fmaxf(fmaxf(x, s[rt][1][1]), s[rt][1][2]);
-                    lm[rt]  = fmaxf(x, s[rt][1][3]);
+                    lm[rt]  = fmaxf(x, s[rt][1][3]) * fac[rt];
                     grow    = grow || lm[rt] > m[rt] + 3.0f;
                 }
                 if (__builtin_amdgcn_ballot_w64(grow) != 0) {
@@ -1170,15 +1171,18 @@ k_fa4_pre(const FaArgs a) {
                     float       p[8];
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        p[e] = __builtin_amdgcn_exp2f(s[rt][e / 4][e % 4] + mu);
+                        p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rt][e / 4][e % 4], fac[rt], mu));
                     }
-                    l[rt] = __builtin_fmaf(((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7])), pinv, l[rt]);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         ph[rt][e] = (_Float16) p[e];
                         if constexpr (OS) {
                             pl[rt][e] = (_Float16) (p[e] - (float) ph[rt][e]);
                         }
+                    }
+                    l[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, ph[rt], l[rt], 0, 0, 0);
+                    if constexpr (OS) {
+                        l[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pl[rt], l[rt], 0, 0, 0);
                     }
                 }
                 // lane m of a group of 16 addresses key m / 4 of the group's 4, positions 4 (m % 4)
@@ -1219,10 +1223,8 @@ k_fa4_pre(const FaArgs a) {
 
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-        float lr = l[rt];
-        lr += __shfl_xor(lr, 16, 64);
-        lr += __shfl_xor(lr, 32, 64);
-        const int r = r0 + (wv * RT + rt) * 16 + c16;
+        const float lr = l[rt][0];
+        const int   r  = r0 + (wv * RT + rt) * 16 + c16;
         if (r >= a.rows) {
             continue;
         }
