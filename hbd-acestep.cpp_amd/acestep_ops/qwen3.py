@@ -73,6 +73,9 @@ def causal_mask(kv_pos, S: int, kv_len: int) -> DTensor:
 
 
 class Qwen3Layer:
+    """The layer's activations lie in buffers that it keeps for the last call's shapes: a captured step
+    is replayed before calls with another number of rows, or on a layer of its own."""
+
     def __init__(self, w_qkv, w_o, w_gate_up, w_down, in_norm_w, post_norm_w, q_norm_w, k_norm_w, H: int, Nh: int,
                  Nkv: int, D: int, I: int, max_seq: int, n_sets: int, kv_type: str = "q8_0", eps: float = 1e-6,
                  rope_theta: float = 1e6, clamp_fp16: bool = False, stream=None, adapters=None, adapter_scales=None):
@@ -99,13 +102,24 @@ class Qwen3Layer:
             self.v_cache = DTensor.zeros((n_sets, Nkv, max_seq, D), "f16")
         else:
             raise ValueError("kv_type: q8_0, q4_0 or f16")
-        self._bufs = {}
+        self._bufs, self._outgrown = {}, []
 
     def _buf(self, name, shape, dtype="f32"):
         b = self._bufs.get(name)
         if b is None or b.shape != tuple(shape):
             b = DTensor.empty(tuple(shape), dtype)
             self._bufs[name] = b
+        return b
+
+    def _work(self, name, need):
+        """At least `need` bytes of workspace. One that a longer call outgrows stays alive, so that a
+        step captured with it (a graph per read length, say) can still be replayed."""
+        b = self._bufs.get(name)
+        if b is None or b.numel() < need:
+            if b is not None:
+                self._outgrown.append(b)
+                need = max(need, 2 * b.numel())
+            b = self._bufs[name] = DTensor.empty((max(need, 256),), "u8")
         return b
 
     def _cache_view(self, c, s0, n, read_len):
@@ -203,7 +217,7 @@ class Qwen3Layer:
         """The rows' low-rank updates of product `name`, added to y in place."""
         if self._adapted(name, ids):
             a, b = self.adapters[name]
-            ws = self._buf("ws_lora_" + name, (max(ops.lora_add_workspace(x, a, b), 16),), "u8")
+            ws = self._work("ws_lora_" + name, ops.lora_add_workspace(x, a, b))
             ops.lora_add(y, x, a, b, ids, self.adapter_scales, out=y, workspace=ws, stream=self.stream)
         return y
 
@@ -255,16 +269,13 @@ class Qwen3Layer:
                                            workspace=self._ws_glu("down", gu), stream=st)
 
     def _ws(self, name, x):
-        need = ops.mul_mat_q8_0_workspace(self.w[name], x)
-        return self._buf("ws_" + name, (max(need, 1),), "u8")
+        return self._work("ws_" + name, ops.mul_mat_q8_0_workspace(self.w[name], x))
 
     def _ws_glu(self, name, gu):
-        need = ops.mul_mat_q8_0_swiglu_workspace(self.w[name], gu)
-        return self._buf("ws_" + name, (max(need, 1),), "u8")
+        return self._work("ws_" + name, ops.mul_mat_q8_0_swiglu_workspace(self.w[name], gu))
 
     def _fa_ws(self, q, k, v):
-        need = ops.flash_attn_workspace(q, k, v)
-        return self._buf("ws_fa", (max(need, 1),), "u8")
+        return self._work("ws_fa", ops.flash_attn_workspace(q, k, v))
 
 
 Qwen3DecodeLayer = Qwen3Layer  # the name the decode-only callers use
@@ -275,15 +286,15 @@ class Qwen3Head:
         """w_out: the vocabulary's Q8 weights in the GGUF layout (repacked here once); norm_w: F32 DTensor."""
         self.V, self.eps, self.stream, self.norm_w = V, eps, stream, norm_w
         self.w = ops.q8_0_repack(w_out, stream=stream)
-        self._bufs = {}
+        self._bufs, self._outgrown = {}, []
 
-    _buf = Qwen3Layer._buf
+    _buf, _work = Qwen3Layer._buf, Qwen3Layer._work
 
     def forward(self, hidden, out=None, **adjust):
         """hidden (N, H) F32 -> logits (N, V): the final norm and the product in one call, then
         ops.logits_adjust in place with the tensors given (history, lengths, penalties, bias,
         allowed, state, err), none of them the bare logits."""
-        ws = self._buf("ws", (max(ops.mul_mat_q8_0_workspace(self.w, hidden), 1),), "u8")
+        ws = self._work("ws", ops.mul_mat_q8_0_workspace(self.w, hidden))
         y = out if out is not None else self._buf("logits", (hidden.shape[0], self.V))
         ops.mul_mat_q8_0_rms_norm(self.w, hidden, self.norm_w, self.eps, out=y, workspace=ws, stream=self.stream)
         if adjust:

@@ -183,3 +183,34 @@ def test_decode_steps_captured_and_replayed(dev):
         st.synchronize()
         for t, w in zip((h, logits, c.layer.k_cache.data, c.layer.v_cache.data), want):
             assert np.array_equal(to_np(t), w, equal_nan=t is logits), f"replay {rep}"
+
+
+@pytest.mark.parametrize("kv_type", ["q4_0", "q8_0"])
+def test_a_graph_per_read_length(dev, kv_type):
+    """Steps captured at growing read lengths, each needing more workspace than the one before, all replayed."""
+    print(f"serving, a graph per read length, {kv_type}", flush=True)
+    st, N, H = Stream(), 2, 256
+    w = {n: orc.quantize_q8_0(randn(s, seed=i, scale=0.05))
+         for i, (n, s) in enumerate({"qkv": (1024, H), "o": (H, 512), "gu": (1024, H), "down": (H, 512)}.items())}
+    layer = Qwen3Layer(*(ops.Q8(to_dev(w[n])) for n in ("qkv", "o", "gu", "down")), *(to_dev(randn((n,), seed=n)) for n in (H, H, 128, 128)),
+                       H, 4, 2, 128, 512, 4096, N, kv_type, EPS, THETA, stream=st.handle)
+    hidden, sets, out = to_dev(randn((N, H), seed=6)), to_dev(np.arange(N, dtype=np.int32)), DTensor.empty((N, H), "f32")
+    steps = []
+    for read in (256, 1024, 4096):
+        pos = np.array([read - 1, read // 2], np.int32)
+        args = (hidden, to_dev(pos), sets, 0, read, decode_mask(pos, read))
+        layer.forward(*args, out=out)
+        st.synchronize()
+        want, g = to_np(out), Graph()
+        with g.capture(st):
+            layer.forward(*args, out=out)
+        steps.append((g, want, args))
+    filler = [DTensor.full_byte((1 << 20,), 0xFF) for _ in range(8)]  # over memory that was given back, were it
+    for rep in range(2):
+        for g, want, _ in steps:
+            out.fill_byte(0xFF)
+            synchronize()
+            g.launch()
+            st.synchronize()
+            assert np.array_equal(to_np(out), want), f"replay {rep}"
+    assert all((to_np(f) == 0xFF).all() for f in filler)
