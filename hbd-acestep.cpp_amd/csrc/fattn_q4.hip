@@ -153,6 +153,13 @@ __device__ __forceinline__ constexpr int fa4_slot(int e) {
     return (e & 2) * 2 + (e & 1) * 2 + (e >> 2);
 }
 
+__device__ __forceinline__ float fa4_max_groups(float v) {  // over the 4 lane groups of 16
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v            = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    const auto t = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(t[0]), __uint_as_float(t[1]));
+}
+
 typedef uint32_t fa4_u2h __attribute__((ext_vector_type(2), aligned(2)));  // 4 mask values
 
 // Query rows (query position, head) of a KV head in tiles of 16, keys split over
@@ -239,8 +246,7 @@ __global__ void __launch_bounds__(64 * W) k_fa4_dec(const FaArgs a) {
             qmax = fmaxf(qmax, fabsf(qv[blk][e]));
         }
     }
-    qmax     = fmaxf(qmax, __shfl_xor(qmax, 16, 64));
-    qmax     = fmaxf(qmax, __shfl_xor(qmax, 32, 64));
+    qmax     = fa4_max_groups(qmax);
     int ex   = (int) (__float_as_uint(qmax) >> 23) - 127;  // 2^ex <= qmax < 2^(ex + 1)
     ex       = ex < -100 ? -100 : ex > 127 ? 10 : ex;      // a row that is not finite: as it is
     const float up = __uint_as_float((uint32_t) (127 + 10 - ex) << 23);
@@ -428,12 +434,11 @@ __global__ void __launch_bounds__(64 * W) k_fa4_dec(const FaArgs a) {
                     mx       = fmaxf(mx, s[mt][r]);
                 }
             }
-            mx                = fmaxf(mx, __shfl_xor(mx, 16, 64));
-            mx                = fmaxf(mx, __shfl_xor(mx, 32, 64));
-            const float mnew  = fmaxf(m, mx);
-            const float mu    = (mnew == -INFINITY ? 0.0f : mnew) - FA4_OFF;
-            if (__builtin_amdgcn_ballot_w64(mnew > m) != 0) {
-                const float al = m == mnew ? 1.0f : __builtin_amdgcn_exp2f(m - mnew);
+            // the maximum that p refers to moves only when a row's grows by more than 2^3: most tiles
+            // need no reduction over lanes
+            if (__builtin_amdgcn_ballot_w64(mx > m + 3.0f) != 0) {
+                const float mnew = fmaxf(m, fa4_max_groups(mx));
+                const float al   = m == mnew ? 1.0f : __builtin_amdgcn_exp2f(m - mnew);
                 l *= al;
 #pragma unroll
                 for (int j = 0; j < 2 * NB; ++j) {
@@ -441,6 +446,7 @@ __global__ void __launch_bounds__(64 * W) k_fa4_dec(const FaArgs a) {
                 }
                 m = mnew;
             }
+            const float mu = (m == -INFINITY ? 0.0f : m) - FA4_OFF;
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
@@ -759,13 +765,6 @@ template <int D, bool OS> struct Fa4P {
     static constexpr int DB = OS ? NB * DS * 4 : 0;
     static constexpr int BUF = KB + VP * VB + DB;
 };
-
-__device__ __forceinline__ float fa4_max_groups(float v) {  // over the 4 lane groups of 16
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v            = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-    const auto t = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return fmaxf(__uint_as_float(t[0]), __uint_as_float(t[1]));
-}
 
 template <int D, bool OS, bool MSK>
 __global__ void __launch_bounds__((64 * Fa4P<D, OS>::W)) __attribute__((amdgpu_waves_per_eu(2)))

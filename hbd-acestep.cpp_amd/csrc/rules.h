@@ -77,19 +77,30 @@ inline bool logits_small_tiles(uint32_t rows, int64_t n_vocab, uint32_t cus) {
     return (int64_t) rows * ((n_vocab + 8191) / 8192) < 4 * (int64_t) cus;
 }
 
-// Attention over Q4_0 K and V: the keys of a row are split over `s` workgroups where that saves
-// more than it costs. A split saves tile_ns of every tile of the row's keys that is left to another
-// workgroup, and costs a launch that joins the results (2300 ns) and the traffic of a partial
-// result, row_ps picoseconds per row and split; `want` workgroups per row are resident at once.
-// us, 128 values, 16 heads on 8, unsplit / split in 2 / 3 / 4 / 6: one row per head of 256 keys 10.4 /
-// 12.0, of 512 13.5 / - / 11.9; 64 positions on 2064 keys 44.7 / 29.4 / 23.8 / 21.6 / 22.8; 512 on
-// 512 23.5 / 34.4; many rows a workgroup: 1024 on 5120 418 / 224 / 162 / 139 / 174
-inline int64_t fa4_splits(int64_t tiles, int64_t rows, int64_t want, int64_t tile_ns, int64_t row_ps) {
-    int64_t s = 1;
-    while (s < want && (s + 1) * (s + 1) * row_ps * rows <= tiles * tile_ns * 1000) {
-        ++s;
+// Attention over Q4_0 K and V: over how many of `items` workgroups each the keys are split, `slots`
+// of them resident at once. A split saves tile_ns of every tile of a row's keys that is left to
+// another workgroup, and costs a launch that joins the results (2300 ns) and the traffic of a partial
+// result, row_ps picoseconds per row and split. us, 128 values, 16 heads on 8, unsplit / split in 2 /
+// 3 / 4 / 6: one row per head of 256 keys 10.4 / 12.0, of 512 13.5 / - / 11.9; 64 positions on 2064
+// keys 44.7 / 29.4 / 23.8 / 21.6 / 22.8; 512 on 512 23.5 / 34.4; many rows a workgroup: 1024 on 5120
+// 418 / 224 / 162 / 139 / 174. Workgroups of a second round are waited for, so one round as full as it
+// gets, or two where they are fuller: 64 sequences of up to 8000 keys, 32 heads on 8 (512 items, 768
+// slots) unsplit 104, in 2 87, in 3 90; 3 of up to 60000 (24 items) in 32 31.6, in 42 35.1
+inline int64_t fa4_splits(int64_t tiles, int64_t rows, int64_t items, int64_t slots, int64_t most, int64_t tile_ns, int64_t row_ps) {
+    int64_t best = 1, least = tiles * tile_ns * ((items + slots - 1) / slots);
+    for (int64_t rounds = 1; rounds <= 2; ++rounds) {
+        const int64_t want = rounds * slots / items < most ? rounds * slots / items : most;
+        int64_t       s    = 1;
+        while (s < want && (s + 1) * (s + 1) * row_ps * rows <= tiles * tile_ns * 1000) {
+            ++s;
+        }
+        const int64_t ns = tiles * tile_ns * ((items * s + slots - 1) / slots) / s + 2300 + row_ps * rows * s / 1000;
+        if (s > 1 && ns < least) {
+            best  = s;
+            least = ns;
+        }
     }
-    return tiles * tile_ns * (s - 1) / s < 2300 + row_ps * rows * s / 1000 ? 1 : s;
+    return best;
 }
 
 struct Fa4Plan {
@@ -111,8 +122,7 @@ inline Fa4Plan fa4_plan(int64_t heads, int64_t rows, int64_t n_kv, int d, bool f
     const int64_t tk = d == 64 ? 64 : 32, tiles = (n_kv + tk - 1) / tk, items = heads * ((rows + 15) / 16);
     const int64_t way = (one ? 1100 : 2200) / 4;  // a tile, one of four waves
     const int64_t most = (tiles + 7) / 8;         // two tiles a wave
-    int64_t       want = (d == 256 ? 1 : 3) * cus / items;
-    Fa4Plan       p{ false, fa4_splits(tiles, all, want < most ? want : most, way, 800) };
+    Fa4Plan       p{ false, fa4_splits(tiles, all, items, (d == 256 ? 1 : 3) * cus, most, way, 800) };
     if (rows <= 32) {
         return p;
     }
@@ -124,9 +134,8 @@ inline Fa4Plan fa4_plan(int64_t heads, int64_t rows, int64_t n_kv, int d, bool f
     const int64_t wgs = heads * ((rows + bq - 1) / bq), slots = cus * (d == 256 || (f32 && d == 128) ? 1 : 2);
     const int64_t ns  = f32 ? (d == 128 ? 5100 : 2600) : (d == 64 ? 1000 : 2000);  // a tile
     const int64_t fit = (tm + 1) / 2;  // two tiles a workgroup
-    want              = slots / wgs;
-    const int64_t s   = fa4_splits(tm, all, want < fit ? want : fit, ns, 250);
-    const int64_t many = 14000 + tm * ns / s * ((wgs * s + slots - 1) / slots) + (s > 1 ? 2300 + all * s / 4 : 0);
+    const int64_t s    = fa4_splits(tm, all, wgs, slots, fit, ns, 250);
+    const int64_t many = 14000 + tm * ns * ((wgs * s + slots - 1) / slots) / s + (s > 1 ? 2300 + all * s / 4 : 0);
     return many < few ? Fa4Plan{ true, s } : p;
 }
 
