@@ -122,7 +122,7 @@ def _p(t):
 
 
 def _s(stream):
-    return ctypes.c_void_p(stream)
+    return stream  # None or a handle: the prototype makes it a pointer
 
 
 def _out(out, shape, dtype):
@@ -227,8 +227,7 @@ def modulate(x, scale, shift, out=None, stream=None):
 
 def get_rows(table, ids, out=None, out_dtype="f32", err=None, stream=None):
     """ggml_get_rows: table (n_rows, n) [or Q8, Q4], ids i32 (n_ids,) -> (n_ids, n)."""
-    n = table.shape[-1]
-    y = _out(out, (ids.shape[0], n), out_dtype)
+    y = out if out is not None else DTensor.empty((ids.shape[0], table.shape[-1]), out_dtype)
     ep = ctypes.c_void_p(err.ptr) if err is not None else None
     _lib.call("mi_get_rows", _p(table), _p(ids), _p(y), ep, _s(stream))
     return y
