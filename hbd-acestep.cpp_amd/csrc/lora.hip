@@ -12,6 +12,7 @@
 // BF16 weights as they are, F16 weights as two exact bf16 parts: three or five products keep
 // everything but 2^-24 of each term, at matrix-core rates that stay far above what the loads need.
 #include "launch.h"
+#include "rules.h"
 
 namespace mi {
 
@@ -85,7 +86,9 @@ __device__ __forceinline__ int32_t lr_id(const LoraArgs & a, uint32_t t) {
     return id < 0 || id >= a.n_ad ? -1 : id;
 }
 
-// h = A x. A workgroup: 16 rows of x (blockIdx.x), one of a.ks shares of the keys (y), rank
+// h = A x. What bounds it: x once (4005 rows of 2560 at rank 32 16.2 us, 2.5 TB/s of x and the shares), or with few
+// rows the chain of ids, weights, products and the sum in LDS (8 rows at rank 16 3.3 us, 48 rows of 24
+// adapters at rank 64 from 4096 keys 7.4 us). A workgroup: 16 rows of x (blockIdx.x), one of a.ks shares of the keys (y), rank
 // block of 16 NR and every a.slots-th distinct adapter of the tile (z). Its 4 waves take
 // alternate steps of 32 keys and are summed in LDS.
 template <int WT, int NR>
@@ -165,7 +168,8 @@ __global__ void __launch_bounds__(256) k_lora_down(const LoraArgs a) {
 
 // y = y0 + B (scale h). A workgroup: 16 TT rows of x (blockIdx.x) and every gridDim.y-th block of
 // 64 NT columns of y, a wave 16 NT of them. h is summed over the key shares, scaled and split
-// once, into LDS; a block's y0 is loaded under the block before it. RS: steps of 32 ranks; U:
+// once, into LDS; a block's y0 is loaded under the block before it. Many rows: memory bounds it
+// (4005 x 19456 at rank 32 136 us, 4.6 TB/s of y0 and y). RS: steps of 32 ranks; U:
 // adapters whose weights are loaded before the first is multiplied. With NT 1 (few rows) the distinct
 // adapters of the tile are shared out over gridDim.z workgroups, each storing the rows of its own
 // (and the first those without one): a row has one adapter, so there is nothing to sum.
@@ -400,13 +404,8 @@ template <int WT, int NR> static void launch_down(const LoraArgs & a, hipStream_
     MI_LAUNCH((k_lora_down<WT, NR>), dim3((a.m + 15) / 16, a.ks, blocks * a.slots), dim3(256), 0, s, a);
 }
 
-// many rows of at least 4 columns: 4 columns of y a lane
-static bool lora_wide(const LoraArgs & a) {
-    return a.m > 64 && a.n >= 4;
-}
-
 template <int WT, int RS> static void launch_up(const LoraArgs & a, hipStream_t s) {
-    if (lora_wide(a)) {
+    if (lora_wide(a.m, a.n)) {
         // rows in tiles of 32 (16 at high ranks), column blocks of 256 over enough workgroups for 8 per CU
         constexpr int  TT    = RS < 8 ? 2 : 1;
         const uint32_t tiles = (a.m + 16 * TT - 1) / (16 * TT), blocks = (a.n + 255) / 256;
@@ -439,7 +438,7 @@ template <int WT> static void launch_w(const LoraArgs & a, hipStream_t s) {
         case 4: launch_up<WT, 4>(a, s); break;
         default: launch_up<WT, 8>(a, s); break;
     }
-    if (lora_wide(a) && a.n % 4 != 0) {
+    if (lora_wide(a.m, a.n) && a.n % 4 != 0) {
         MI_LAUNCH(k_lora_up_rest, dim3((uint32_t) (((uint64_t) a.m * (a.n & 3u) + 255) / 256)), dim3(256), 0, s, a,
                   WT == MI_TYPE_F16 ? 1 : 0);
     }

@@ -77,6 +77,17 @@ inline bool logits_small_tiles(uint32_t rows, int64_t n_vocab, uint32_t cus) {
     return (int64_t) rows * ((n_vocab + 8191) / 8192) < 4 * (int64_t) cus;
 }
 
+// Adapters' second product, m rows of n columns: whether a lane takes 4 columns of each of its rows, in
+// tiles of 32 rows (16 at high ranks) and 256 columns, not one column in tiles of 16 rows and 64
+// columns whose adapters are shared out over workgroups. Wide tiles move y at the rate of memory; small
+// ones give every adapter of few rows a workgroup (us wide / narrow, both products: 64 x 6144, 8
+// adapters 17.7 / 12.6; 200 x 6144 21.1 / 18.2; 500 x 6144 32.4 / 36.0; 64 x 19456, one 13.2 / 12.6;
+// 100 x 19456 15.1 / 16.6; 200 x 2560, 24 adapters of rank 64 64.0 / 38.5; 1000 x 1024 12.9 / 12.0; 600 x
+// 2560 14.6 / 15.5; 2000 x 19456, 16 in turn 248 / 309; 1000 x 6144, 24 in turn 84.4 / 77.9).
+inline bool lora_wide(int64_t m, int64_t n) {
+    return n >= 4 && m * n >= 1500000;
+}
+
 // Attention over Q4_0 K and V: over how many of `items` workgroups each the keys are split, `slots`
 // of them resident at once. A split saves tile_ns of every tile of a row's keys that is left to
 // another workgroup, and costs a launch that joins the results (2300 ns) and the traffic of a partial

@@ -72,10 +72,23 @@ def test_adapters_of_many_rows_and_ranks(dev, m, k, n, r, e, dt):
     assert np.array_equal(got, run_lora(x, y0, a, b, ids, scales, out="y0"))
 
 
+@pytest.mark.parametrize("run", [1, 37, 400])
+@pytest.mark.parametrize("m,k,n,r,e,dt", [(1500, 32, 1030, 33, 40, "f16"), (1500, 64, 1027, 256, 3, "bf16"), (1600, 32, 1001, 100, 9, "bf16"),
+                                          (1501, 96, 1000, 16, 5, "f16"), (3100, 64, 515, 64, 7, "bf16"), (1505, 32, 1002, 129, 2, "f16")])
+def test_adapters_of_wide_tiles(dev, m, k, n, r, e, dt, run):
+    """Enough rows and columns for the kernel with 4 columns a lane, runs of one adapter, columns that are no whole 4."""
+    print(f"lora wide m={m} k={k} n={n} r={r} e={e} {dt} run={run}", flush=True)
+    ids = np.repeat(rng(m).integers(-1, e, (m + run - 1) // run), run)[:m]
+    x, y0, a, ah, b, bh, ids, scales = lora_case(m, k, n, r, e, dt, seed=m + r, ids=ids)
+    got = run_lora(x, y0, a, b, ids, scales)
+    check_lora(got, y0, x, ah, bh, ids, scales)
+    assert np.array_equal(got, run_lora(x, y0, a, b, ids, scales, out="y0"))
+
+
 def test_adapters_in_place_on_columns_of_a_wider_buffer(dev):
     """Two products' columns of one buffer take their own adapters in place; x with outer dimensions."""
     print("lora, columns of a wider buffer", flush=True)
-    for m in (12, 90):
+    for m in (12, 90, 16000):
         x, y0, a, ah, b, bh, ids, scales = lora_case(m, 64, 96, 16, 4, "bf16", seed=m)
         wide = np.concatenate([randn((m, 33), seed=1), y0, randn((m, 40), seed=2)], 1)
         wd = to_dev(wide)

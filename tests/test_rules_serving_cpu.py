@@ -6,6 +6,12 @@ LOGITS = [  # rows, tokens, us in tiles of 2048, of 4096
     (8, 151669, 6.0, 6.8), (64, 151669, 19.5, 18.5),
 ]
 
+ADAPTERS = [  # rows, columns, us wide, us narrow
+    (32, 6144, 15.6, 11.4), (64, 6144, 17.7, 12.6), (100, 6144, 18.3, 15.0), (200, 6144, 21.1, 18.2), (500, 6144, 32.4, 36.0),
+    (100, 19456, 15.1, 16.6), (200, 19456, 20.0, 22.9), (200, 2560, 64.0, 38.5), (4000, 2560, 246.3, 285.6), (2000, 19456, 247.7, 309.0),
+    (600, 2560, 14.6, 15.5), (1000, 1024, 12.9, 12.0), (4000, 1024, 26.5, 32.7), (150, 19456, 42.0, 57.1), (80, 19456, 12.0, 13.4),
+]
+
 ATTENTION = [  # KV heads and sequences, rows of each, keys, values of a head, F32 y, us 16 rows a workgroup, us many
     (8, 66, 33, 128, 1, 9.9, 19.4), (8, 66, 33, 128, 0, 9.4, 15.2), (8, 128, 464, 128, 1, 13.3, 22.8), (8, 128, 464, 128, 0, 12.5, 18.8),
     (8, 514, 387, 128, 1, 18.9, 35.4), (8, 514, 387, 128, 0, 16.8, 24.2), (8, 1024, 512, 128, 1, 23.5, 34.8),
@@ -28,6 +34,12 @@ SPLITS = [  # KV heads and sequences, rows of each, keys, least and most splits 
 def test_logits_take_the_quicker_tiles(tmp_path):
     got = _run(tmp_path, lambda r: f"logits_small_tiles({r[0]}, {r[1]}, 256)", LOGITS)
     assert got == [int(r[2] < r[3]) for r in LOGITS]
+
+
+def test_adapters_take_the_quicker_tiles(tmp_path):
+    got = _run(tmp_path, lambda r: f"lora_wide({r[0]}, {r[1]})", ADAPTERS)
+    bad = [r for r, g in zip(ADAPTERS, got) if g != (r[2] < r[3])]
+    assert not bad, bad
 
 
 def test_attention_takes_the_quicker_kernel(tmp_path):
