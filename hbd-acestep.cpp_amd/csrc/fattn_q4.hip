@@ -175,6 +175,13 @@ typedef uint32_t fa4_u2h __attribute__((ext_vector_type(2), aligned(2)));  // 4 
 // The raw blocks of the next tile are in flight under the current one's math. Tiles with
 // no live key are not read where the 16 rows share a mask row (one query position), and
 // a key that no row attends to counts as v = 0 whatever its bytes are.
+// Bound by a tile's chain and its unpacking: a lone wave takes 1.5 us a tile (D = 128, BF16 y; F32 1.6),
+// three on a SIMD 2.1 for a tile each. Three waves a SIMD (F32 y, a mask row each, left to itself takes 171
+// registers and two waves: 5 positions on 20000 46.4 us instead of 39.0, 16 on 4016 66.4 instead of 55.9), two at
+// D = 256 (one: 7 positions on 30177, BF16 y, 63 us instead of 52; 8 rows on 3001 23.3 instead of 24.0). 2 rows
+// of 60013 keys, 32 heads on 8, 128, BF16 y: 29 us, 3.7 TB/s; 8 of up to 6600, F32 y: 21 us, 1.8 TB/s.
+// Tiles of 64 keys at D = 128 leave half as many waves a turn; 8 waves a workgroup: 257 positions on
+// 387 keys 25.8 us instead of 19.0, 64 on 2064 29.6 instead of 22.8.
 template <int D> struct Fa4 {
     static constexpr int NB   = D / 32;
     static constexpr int TK   = D == 64 ? 64 : 32;  // keys per tile
@@ -196,7 +203,8 @@ template <int D> struct Fa4 {
 
 // OS: F32 y (parts of q, P and V); MS: 0 no mask, 1 one mask row for all rows of the tile, 2 a mask row each
 template <int D, bool OS, int MS, int W>
-__global__ void __launch_bounds__(64 * W) k_fa4_dec(const FaArgs a) {
+__global__ void __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 256 ? 2 : D == 128 && OS && MS == 2 ? 3 : 1)))
+k_fa4_dec(const FaArgs a) {
     using F           = Fa4<D>;
     constexpr int QP  = OS ? 2 : 1;
     constexpr int NB  = F::NB, TK = F::TK, IPL = F::IPL, MT = F::MT;
@@ -749,7 +757,12 @@ __global__ void __launch_bounds__(256) k_fa4_combine_few(const FaArgs a) {
 // block that is not finite the keys that no row of the workgroup attends to count as zeros. The
 // waves tell each other at the barrier before they lay the tile out.
 // The maximum that p refers to moves only when a row's grows by more than 2^3, so most tiles
-// need no reduction over lanes. Masks are looked up per tile in k_fa_mask_summary's bytes.
+// need no reduction over lanes; the row sums are products with ones. Masks are looked up per tile in
+// k_fa_mask_summary's bytes.
+// Bound by unpacking and exponentials beside the matrix cores (busy 28 % of the cycles; two waves a
+// SIMD is what the registers leave). 8 x 2048 positions, 32 heads on 8, 128: BF16 y without a mask
+// 642 us, 856 TFLOP/s, causal 381 and 16 for the summary; F32 y 1292 and 752. 8 waves (256 rows) in BF16:
+// 626 without a mask, but 2048 positions on 6144 keys 239 instead of 229.
 template <int D, bool OS> struct Fa4P {
     static constexpr int NB = D / 32;
     static constexpr int T  = D == 256 ? 32 : 64;       // keys per tile

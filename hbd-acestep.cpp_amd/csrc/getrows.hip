@@ -276,7 +276,8 @@ __global__ void __launch_bounds__(256) k_get_rows_q8_0_flat(const GetRowsArgs a,
 // Q4_0 rows: y = (q - 8) * d, exact in fp32 (4 + 11 significant bits). Flat, as above: a thread
 // makes one 16-byte store per step, whole lines per store instruction, from OPS consecutive
 // nibbles of one half of a block (one load at the levels' 2-byte alignment; the other half's
-// thread reads the same bytes again, from the cache).
+// thread reads the same bytes again, from the cache). Memory bounds it: 131072 rows of 128 to bf16
+// 8.2 us, 5.2 TB/s; with a thread writing its 8 bytes' low and high nibbles, 16 values apart, 15.2.
 typedef uint32_t gr_u2 __attribute__((ext_vector_type(2), aligned(2)));
 typedef uint32_t gr_u1 __attribute__((aligned(2)));
 

@@ -133,17 +133,19 @@ inline Fa4Plan fa4_plan(int64_t heads, int64_t rows, int64_t n_kv, int d, bool f
     const int64_t tk = d == 64 ? 64 : 32, tiles = (n_kv + tk - 1) / tk, items = heads * ((rows + 15) / 16);
     const int64_t way = (one ? 1100 : 2200) / 4;  // a tile, one of four waves
     const int64_t most = (tiles + 7) / 8;         // two tiles a wave
-    Fa4Plan       p{ false, fa4_splits(tiles, all, items, (d == 256 ? 1 : 3) * cus, most, way, 800) };
+    const int64_t room = (d == 256 ? 2 : 3) * cus;  // resident workgroups
+    Fa4Plan       p{ false, fa4_splits(tiles, all, items, room, most, way, 800) };
     if (rows <= 32) {
         return p;
     }
-    const int64_t work = (f32 ? 12 : 9) * items * p.splits + (f32 ? 142 : 108) * (d == 256 ? 2 : 1) * items * tiles / 100;
-    const int64_t last = tiles * way / p.splits;
+    int64_t       work = (f32 ? 12 : 9) * items * p.splits + (f32 ? 142 : 108) * (d == 256 ? 7 : 4) * items * tiles / 400;
+    const int64_t last = tiles * way / p.splits, wg = items * p.splits;
+    work = wg <= room ? work : work / wg * ((wg + room - 1) / room * room);  // a last round that is not full
     const int64_t few  = 8500 + (work > last ? work : last) + (p.splits > 1 ? 2300 + all * p.splits * 8 / 10 : 0);
     // many
     const int64_t bq = f32 && d == 128 ? 256 : 128, tkm = d == 256 ? 32 : 64, tm = (n_kv + tkm - 1) / tkm;
     const int64_t wgs = heads * ((rows + bq - 1) / bq), slots = cus * (d == 256 || (f32 && d == 128) ? 1 : 2);
-    const int64_t ns  = f32 ? (d == 128 ? 5100 : 2600) : (d == 64 ? 1000 : 2000);  // a tile
+    const int64_t ns  = f32 ? (d == 64 ? 2600 : d == 128 ? 5100 : 3400) : (d == 64 ? 1000 : d == 128 ? 2000 : 1600);  // a tile
     const int64_t fit = (tm + 1) / 2;  // two tiles a workgroup
     const int64_t s    = fa4_splits(tm, all, wgs, slots, fit, ns, 250);
     const int64_t many = 14000 + tm * ns * ((wgs * s + slots - 1) / slots) / s + (s > 1 ? 2300 + all * s / 4 : 0);

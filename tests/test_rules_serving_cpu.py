@@ -21,8 +21,10 @@ ATTENTION = [  # KV heads and sequences, rows of each, keys, values of a head, F
     (64, 512, 128, 128, 1, 44.7, 28.2), (64, 512, 128, 128, 0, 35.0, 16.9), (64, 1028, 257, 128, 1, 126.8, 52.3),
     (8, 1024, 8256, 128, 1, 193.2, 112.4), (24, 400, 600, 64, 0, 19.8, 25.1), (24, 400, 600, 64, 1, 27.1, 36.6),
     (8, 514, 387, 64, 1, 12.8, 33.0), (64, 512, 128, 64, 0, 25.7, 13.9), (64, 256, 4064, 64, 1, 129.6, 73.6),
-    (8, 128, 2064, 256, 1, 33.5, 232.1), (8, 4096, 2048, 256, 0, 297.2, 118.2), (64, 512, 128, 256, 1, 128.0, 34.5),
-    (8, 1024, 512, 256, 1, 55.9, 42.5), (8, 1024, 512, 256, 0, 35.4, 40.8),
+    (8, 4096, 2048, 256, 0, 288.8, 117.5), (64, 512, 128, 256, 1, 84.6, 34.0), (64, 512, 128, 256, 0, 75.3, 22.3),
+    (8, 514, 387, 256, 1, 33.1, 41.2), (8, 514, 387, 256, 0, 27.1, 34.5), (24, 400, 600, 256, 0, 58.0, 37.8), (24, 400, 600, 256, 1, 68.2, 55.4),
+    (64, 64, 4016, 256, 0, 79.8, 68.7), (64, 64, 4016, 256, 1, 98.9, 127.3), (8, 128, 464, 256, 1, 20.9, 29.2), (8, 128, 464, 256, 0, 19.7, 23.2),
+    (8, 80, 5040, 256, 1, 46.2, 42.4), (8, 80, 5040, 256, 0, 39.8, 32.1), (8, 2048, 1024, 256, 1, 113.5, 82.3),
 ]
 
 SPLITS = [  # KV heads and sequences, rows of each, keys, least and most splits that came within 12 % of the best
