@@ -1022,16 +1022,17 @@ def gemv_bench(steps: int):
 
 # ---------------------------------------------------------------------------
 # One whole Qwen3-4B decoder layer on the device (reported with --decode-layer):
-# batch 8, Q8_0 weights, an F16 KV cache (the LM's own, qwen3-lm.h:190-191) and a
-# Q8_0 one, 8192 slots per sequence, lengths U[1, 8192] and the 256-bucketed read
+# batch 8, Q8_0 weights, an F16 KV cache (the LM's own, qwen3-lm.h:190-191), a Q8_0 one
+# and a Q4_0 one (also with an adapter of rank 16 per sequence on all four products), 8192 slots per sequence, lengths U[1, 8192] and the 256-bucketed read
 # (qw3lm_forward_batch, qwen3-lm.h:626-741). One JSON line per cache type.
 # ---------------------------------------------------------------------------
 def decode_layer_bench(steps: int):
-    for kv_type in ("f16", "q8_0"):
+    for kv_type in ("f16", "q8_0", "q4_0"):
         decode_layer_bench_kv(steps, kv_type)
+    decode_layer_bench_kv(steps, "q4_0", rank=16)
 
 
-def decode_layer_bench_kv(steps: int, kv_type: str):
+def decode_layer_bench_kv(steps: int, kv_type: str, rank: int = 0):
     from acestep_ops import device, ops
     from acestep_ops.device import DTensor, Event, Graph, Stream
     from acestep_ops.qwen3 import Qwen3DecodeLayer, decode_mask
@@ -1054,13 +1055,20 @@ def decode_layer_bench_kv(steps: int, kv_type: str):
     ones = lambda n: DTensor.from_numpy(np.ones(n, np.float32))  # noqa: E731
     layer = Qwen3DecodeLayer(q8w((Nh + 2 * Nkv) * D, H), q8w(H, Nh * D), q8w(2 * I, H), q8w(H, I), ones(H), ones(H),
                              ones(D), ones(D), H, Nh, Nkv, D, I, SLOTS, N, kv_type, stream=sh)
-    if kv_type == "q8_0":
-        kb = np.zeros((N, Nkv, SLOTS, D // 32 * 34), np.uint8)
+    ids = None
+    if rank:
+        ids = DTensor.from_numpy(np.arange(N, dtype=np.int32))
+        for name, w in layer.w.items():
+            layer.adapters[name] = tuple(DTensor.from_numpy(rng.integers(0x3C00, 0x3D00, s, dtype=np.uint16), "bf16")
+                                         for s in ((N, rank, w.k), (N, w.n, rank)))  # bf16 of 0.008 to 0.03
+    if kv_type in ("q8_0", "q4_0"):
+        wrap, nb = (ops.Q8, 34) if kv_type == "q8_0" else (ops.Q4, 18)
+        kb = np.zeros((N, Nkv, SLOTS, D // 32 * nb), np.uint8)
         kb[..., 2:] = rng.integers(-127, 128, kb[..., 2:].shape, dtype=np.int8).view(np.uint8)
-        kb.reshape(-1, 34)[:, :2] = np.full((kb.size // 34, 1), 1e-2, np.float16).view(np.uint8)
-        layer.k_cache = ops.Q8(DTensor.from_numpy(kb))
-        layer.v_cache = ops.Q8(DTensor.from_numpy(kb))
-        row_bytes = D // 32 * 34
+        kb.reshape(-1, nb)[:, :2] = np.full((kb.size // nb, 1), 1e-2, np.float16).view(np.uint8)
+        layer.k_cache = wrap(DTensor.from_numpy(kb))
+        layer.v_cache = wrap(DTensor.from_numpy(kb))
+        row_bytes = D // 32 * nb
     else:
         kh = rng.standard_normal((N, Nkv, SLOTS, D), dtype=np.float32).astype(np.float16)
         layer.k_cache = DTensor.from_numpy(kh.view(np.uint16), "f16")
@@ -1071,12 +1079,12 @@ def decode_layer_bench_kv(steps: int, kv_type: str):
     out = DTensor.empty((N, H), "f32")
     dpos, dsets = DTensor.from_numpy(pos), DTensor.from_numpy(np.arange(N, dtype=np.int32))
     mask = decode_mask(pos, read)
-    layer.forward(hidden, dpos, dsets, 0, read, mask, out=out)
+    layer.forward(hidden, dpos, dsets, 0, read, mask, out=out, adapter_ids=ids)
     st.synchronize()
     g = Graph()
     with g.capture(st):
         for _ in range(steps):
-            layer.forward(hidden, dpos, dsets, 0, read, mask, out=out)
+            layer.forward(hidden, dpos, dsets, 0, read, mask, out=out, adapter_ids=ids)
     g.launch()
     st.synchronize()
     e0, e1 = Event(), Event()
@@ -1086,11 +1094,14 @@ def decode_layer_bench_kv(steps: int, kv_type: str):
     e1.synchronize()
     us = 1000.0 * e0.elapsed_ms(e1) / steps
     wbytes = sum(w.n * (w.k // 32) * 34 for w in layer.w.values())
+    wbytes += sum(2 * N * rank * (w.n + w.k) for w in layer.w.values())
     # K/V bytes the step must read: each sequence's live keys (the mask's -inf tail
     # of the 256-bucketed read is skipped before any byte of it is loaded).
     kvb = int(lens.sum()) * Nkv * row_bytes * 2
     print(json.dumps({"config": f"Qwen3-4B decode layer, batch {N}, Q8_0 weights, {kv_type.upper()} KV cache ({SLOTS} "
-                                f"slots, lengths U[1,{SLOTS}], read {read}), every op on the device",
+                                f"slots, lengths U[1,{SLOTS}], read {read})"
+                                + (f", an adapter of rank {rank} per sequence on every product" if rank else "")
+                                + ", every op on the device",
                       "us_per_layer": round(us, 2), "weight_bytes": wbytes, "kv_bytes_live": kvb,
                       "GB/s": round((wbytes + kvb) / (us * 1e-6) / 1e9, 1),
                       "frac": round((wbytes + kvb) / (us * 1e-6) / 1e9 / HBM_PEAK_GBS, 3),
@@ -1103,14 +1114,14 @@ def decode_layer_bench_kv(steps: int, kv_type: str):
 # One whole Qwen3-4B decoder layer in prefill on the device (reported with
 # --prefill-layer): the two CFG sequences (conditional and unconditional KV
 # sets, qwen3-lm.h:429-431) of a 512-token prompt from slot 0, Q8_0 weights,
-# an F16 KV cache (the LM's own, qwen3-lm.h:190-191) and a Q8_0 one
+# an F16 KV cache (the LM's own, qwen3-lm.h:190-191), a Q8_0 and a Q4_0 one
 # (qw3lm_forward, qwen3-lm.h:429-549). One JSON line per cache type.
 # ---------------------------------------------------------------------------
 def prefill_layer_bench(steps: int):
     # the CFG pair of a 512-token prompt, and the batched prefill of 8 sequences
     # x 2048 tokens (the Qwen3-4B batch-8 prefill into a KV cache)
     for n, s_, slots in ((2, 512, 4096), (8, 2048, 8192)):
-        for kv_type in ("f16", "q8_0"):
+        for kv_type in ("f16", "q8_0", "q4_0"):
             prefill_layer_bench_kv(steps, kv_type, n, s_, slots)
 
 
