@@ -201,7 +201,9 @@ int mi_cpy_q8_0(const mi_tensor * src, const mi_tensor * dst, int rounding, mi_s
  *   pos0:       I32 [B]   first slot written for sequence b
  *   sets:       I32 [B] or NULL (set = b)
  * cache[:, pos0[b] + t, h, sets[b]] = k[:, h, t, b]. Out-of-range slots or
- * sets are skipped and counted in *d_err when d_err != NULL. */
+ * sets are skipped and counted in *d_err when d_err != NULL. A slot that two
+ * sequences of one call name is written by both at once (a Q8_0 or Q4_0 block
+ * may end up with the scale of one and levels of the other). */
 int mi_kv_store(const mi_tensor * k, const mi_tensor * k_cache, const mi_tensor * v, const mi_tensor * v_cache,
                 const mi_tensor * pos0, const mi_tensor * sets, int rounding, int32_t * d_err, mi_stream stream);
 
