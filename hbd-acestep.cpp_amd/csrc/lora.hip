@@ -229,33 +229,52 @@ __global__ void __launch_bounds__(256) k_lora_up(const LoraArgs a) {
     };
     uint32_t n0 = (blockIdx.y * 4 + wv) * (16 * NT);
     load(n0);
-    for (int i = threadIdx.x; i < R * RS * 32; i += 256) {
-        const int      t = i / (RS * 32), r = i - t * RS * 32;
-        const int32_t  it  = __shfl(idl, t, 64);
-        const bool     on  = it >= 0 && r < (int) a.r && (NT != 1 || own >> t & 1);
-        const uint32_t tr  = t0 + t < a.m ? t0 + t : a.m - 1;
-        const float *  hp  = a.h + (int64_t) tr * a.rp + (r < (int) a.r ? r : 0);
-        const int64_t  st  = (int64_t) a.m * a.rp;
-        const float    sc  = a.scales && on ? *(const float *) (a.scales + (int64_t) it * a.s0) : 1.0f;
-        float          v   = 0.0f;
-        for (uint32_t s = 0; on && s < a.ks; s += 16) {  // 16 shares in flight
-            float p[16];
+    // G elements a thread and 16 key shares of each in flight
+    constexpr int E = R * RS * 32 / 256, G = E < 4 ? E : 4;
+    for (int i0 = threadIdx.x; i0 < R * RS * 32; i0 += 256 * G) {
+        const float * hp[G];
+        bool          on[G], any = false;
+        float         sc[G], v[G];
 #pragma unroll
-            for (int q = 0; q < 16; ++q) {
-                p[q] = hp[(s + q < a.ks ? s + q : a.ks - 1) * st];
+        for (int g = 0; g < G; ++g) {
+            const int      i = i0 + 256 * g, t = i / (RS * 32), r = i - t * RS * 32;
+            const int32_t  it = __shfl(idl, t, 64);
+            const uint32_t tr = t0 + t < a.m ? t0 + t : a.m - 1;
+            on[g] = it >= 0 && r < (int) a.r && (NT != 1 || own >> t & 1);
+            any   = any || on[g];
+            hp[g] = a.h + (int64_t) tr * a.rp + (r < (int) a.r ? r : 0);
+            sc[g] = a.scales && on[g] ? *(const float *) (a.scales + (int64_t) it * a.s0) : 1.0f;
+            v[g]  = 0.0f;
+        }
+        const int64_t st = (int64_t) a.m * a.rp;
+        for (uint32_t s = 0; any && s < a.ks; s += 16) {
+            float p[G][16];
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+#pragma unroll
+                for (int q = 0; q < 16; ++q) {  // past the last share: it again; rows without an adapter hold anything
+                    p[g][q] = hp[g][(s + q < a.ks ? s + q : a.ks - 1) * st];
+                }
             }
 #pragma unroll
-            for (int q = 0; q < 16; ++q) {
-                v += s + q < a.ks ? p[q] : 0.0f;
+            for (int g = 0; g < G; ++g) {
+#pragma unroll
+                for (int q = 0; q < 16; ++q) {
+                    v[g] += s + q < a.ks ? p[g][q] : 0.0f;
+                }
             }
         }
-        v = on ? v * sc : 0.0f;
-        const __bf16 p0 = (__bf16) v;
-        const float  r0 = v - (float) p0;
-        const __bf16 p1 = (__bf16) r0;
-        hs[t * RQ + r]           = p0;
-        hs[(R + t) * RQ + r]     = p1;
-        hs[(2 * R + t) * RQ + r] = (__bf16) (r0 - (float) p1);
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            const int    i = i0 + 256 * g, t = i / (RS * 32), r = i - t * RS * 32;
+            const float  x = on[g] ? v[g] * sc[g] : 0.0f;
+            const __bf16 x0 = (__bf16) x;
+            const float  r0 = x - (float) x0;
+            const __bf16 x1 = (__bf16) r0;
+            hs[t * RQ + r]           = x0;
+            hs[(R + t) * RQ + r]     = x1;
+            hs[(2 * R + t) * RQ + r] = (__bf16) (r0 - (float) x1);
+        }
     }
     __syncthreads();
     const bool vec = a.r % 8 == 0;
