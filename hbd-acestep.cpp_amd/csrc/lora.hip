@@ -425,10 +425,12 @@ template <int WT, int NR> static void launch_down(const LoraArgs & a, hipStream_
 
 template <int WT, int RS> static void launch_up(const LoraArgs & a, hipStream_t s) {
     if (lora_wide(a.m, a.n)) {
-        // rows in tiles of 32 (16 at high ranks), column blocks of 256 over enough workgroups for 8 per CU
+        // rows in tiles of 32 (16 at high ranks), column blocks of 256 over enough workgroups for 6 per CU (both
+        // products, us, for 3 / 4 / 6 / 8 / 12: 4005 x 19456 155.4 / 158.2 / 153.0 / 154.9 / 156.6; 793 x 19456 41.3 / 40.7 /
+        // 41.9 / 43.5 / 43.4; 1500 x 19456 65.2 / 62.2 / 63.0 / 63.1 / 65.4)
         constexpr int  TT    = RS < 8 ? 2 : 1;
         const uint32_t tiles = (a.m + 16 * TT - 1) / (16 * TT), blocks = (a.n + 255) / 256;
-        const uint32_t want  = ((uint32_t) num_cus() * 8 + tiles - 1) / tiles;
+        const uint32_t want  = ((uint32_t) num_cus() * 6 + tiles - 1) / tiles;
         MI_LAUNCH((k_lora_up<WT, 4, TT, RS, 1>), dim3(tiles, want < blocks ? want : blocks), dim3(256), 0, s, a);
     } else {
         // the adapters of a tile over enough workgroups for 2 per CU (48 rows of 24 adapters, 2560
