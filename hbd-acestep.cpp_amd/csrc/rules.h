@@ -81,9 +81,9 @@ inline bool logits_small_tiles(uint32_t rows, int64_t n_vocab, uint32_t cus) {
 // tiles of 32 rows (16 at high ranks) and 256 columns, not one column in tiles of 16 rows and 64
 // columns whose adapters are shared out over workgroups. Wide tiles move y at the rate of memory; small
 // ones give every adapter of few rows a workgroup (us wide / narrow, both products: 64 x 6144, 8
-// adapters 17.7 / 12.6; 200 x 6144 21.1 / 18.2; 500 x 6144 32.4 / 36.0; 64 x 19456, one 13.2 / 12.6;
-// 100 x 19456 15.1 / 16.6; 200 x 2560, 24 adapters of rank 64 64.0 / 38.5; 1000 x 1024 12.9 / 12.0; 600 x
-// 2560 14.6 / 15.5; 2000 x 19456, 16 in turn 248 / 309; 1000 x 6144, 24 in turn 84.4 / 77.9).
+// adapters 16.5 / 11.7; 200 x 6144 19.6 / 16.7; 500 x 6144 30.7 / 34.1; 64 x 19456, one 11.4 / 11.7;
+// 100 x 19456 13.1 / 14.9; 200 x 2560, 24 adapters of rank 64 62.9 / 36.0; 1000 x 1024 11.4 / 11.3; 600 x
+// 2560 12.9 / 14.6; 2000 x 19456, 16 in turn 249 / 291; 1000 x 6144, 24 in turn 82.5 / 73.8).
 inline bool lora_wide(int64_t m, int64_t n) {
     return n >= 4 && m * n >= 1500000;
 }

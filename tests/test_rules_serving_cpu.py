@@ -7,9 +7,9 @@ LOGITS = [  # rows, tokens, us in tiles of 2048, of 4096
 ]
 
 ADAPTERS = [  # rows, columns, us wide, us narrow
-    (32, 6144, 15.6, 11.4), (64, 6144, 17.7, 12.6), (100, 6144, 18.3, 15.0), (200, 6144, 21.1, 18.2), (500, 6144, 32.4, 36.0),
-    (100, 19456, 15.1, 16.6), (200, 19456, 20.0, 22.9), (200, 2560, 64.0, 38.5), (4000, 2560, 246.3, 285.6), (2000, 19456, 247.7, 309.0),
-    (600, 2560, 14.6, 15.5), (1000, 1024, 12.9, 12.0), (4000, 1024, 26.5, 32.7), (150, 19456, 42.0, 57.1), (80, 19456, 12.0, 13.4),
+    (32, 6144, 14.5, 10.1), (64, 6144, 16.5, 11.7), (100, 6144, 17.1, 13.9), (200, 6144, 19.6, 16.7), (500, 6144, 30.7, 34.1),
+    (100, 19456, 13.1, 14.9), (200, 19456, 18.1, 20.7), (200, 2560, 62.9, 36.0), (4000, 2560, 238.1, 268.4), (2000, 19456, 248.5, 290.6),
+    (600, 2560, 12.9, 14.6), (4000, 1024, 24.7, 30.2), (150, 19456, 39.9, 50.2), (80, 19456, 10.8, 12.4),
 ]
 
 ATTENTION = [  # KV heads and sequences, rows of each, keys, values of a head, F32 y, us 16 rows a workgroup, us many
