@@ -568,8 +568,8 @@ k_fa4_dec(const FaArgs a) {
             }
 #pragma unroll
             for (int w = 0; w < W; ++w) {
-                const float mw = stat[w][r][0];
-                ls += mw == -INFINITY ? 0.0f : stat[w][r][1] * __builtin_amdgcn_exp2f(mw - mr2);
+                const float mw = stat[w][r][0];  // -inf without a live score, or with NaN alone: l is 0 or NaN
+                ls += stat[w][r][1] * (mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mw - mr2));
             }
             const int rr = rt * 16 + r;
             if (a.splits > 1) {
@@ -597,6 +597,8 @@ k_fa4_dec(const FaArgs a) {
 // exp2(m_i - max m). A workgroup per row: D / 4 lanes take a float4 of the columns, the groups of
 // them every SG-th split. The outputs of the first PRE splits of each group are loaded with the
 // (m, l), before the weights are known: one round of memory latency for up to SG * PRE splits.
+// A split without a live score has m = -inf and zeros; one whose live scores are all NaN has m = -inf
+// too, and NaN: every split is added, with weight 0 as well, so that its NaN shows.
 constexpr int FA4_MAX_SPLITS = 1024;
 
 template <int D, int PRE>
@@ -615,7 +617,7 @@ __global__ void __launch_bounds__(256) k_fa4_combine(const FaArgs a) {
     const float *  p = a.ws + (int64_t) rec * a.splits * (D + 4);
     fa4_f4         pv[PRE];
 #pragma unroll
-    for (int j = 0; j < PRE; ++j) {  // past the last split: the last one again, weight 0
+    for (int j = 0; j < PRE; ++j) {  // past the last split: the last one again, never added
         const int s = sg + SG * j;
         pv[j]       = *(const fa4_f4 *) (p + (int64_t) (s < last ? s : last) * (D + 4) + 4 + 4 * c);
     }
@@ -625,7 +627,7 @@ __global__ void __launch_bounds__(256) k_fa4_combine(const FaArgs a) {
         const int    s = tid + 256 * i;
         const float2 x = *(const float2 *) (p + (int64_t) (s < last ? s : last) * (D + 4));
         ml[i]          = s <= last ? x.x : -INFINITY;
-        ll[i]          = x.y;
+        ll[i]          = s <= last ? x.y : 0.0f;
         m              = fmaxf(m, ml[i]);
     }
     m = group_max<64>(m);
@@ -639,7 +641,7 @@ __global__ void __launch_bounds__(256) k_fa4_combine(const FaArgs a) {
         const int   s = tid + 256 * i;
         const float w = ml[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml[i] - m);
         wsh[s]        = w;
-        l             = w == 0.0f ? l : __builtin_fmaf(w, ll[i], l);
+        l             = __builtin_fmaf(w, ll[i], l);
     }
     l = group_sum<64>(l);
     if ((tid & 63) == 0) {
@@ -650,10 +652,11 @@ __global__ void __launch_bounds__(256) k_fa4_combine(const FaArgs a) {
     fa4_f4 acc = { 0.0f, 0.0f, 0.0f, 0.0f };
 #pragma unroll
     for (int j = 0; j < PRE; ++j) {
-        const float w = wsh[sg + SG * j];
+        const int   s = sg + SG * j;
+        const float w = wsh[s];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            acc[e] = w == 0.0f ? acc[e] : __builtin_fmaf(w, pv[j][e], acc[e]);
+            acc[e] = s <= last ? __builtin_fmaf(w, pv[j][e], acc[e]) : acc[e];
         }
     }
     for (int s0 = SG * PRE + sg; s0 <= last; s0 += SG * PRE) {
@@ -668,7 +671,7 @@ __global__ void __launch_bounds__(256) k_fa4_combine(const FaArgs a) {
             const float w = s <= last ? wsh[s] : 0.0f;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                acc[e] = w == 0.0f ? acc[e] : __builtin_fmaf(w, pv[j][e], acc[e]);
+                acc[e] = s <= last ? __builtin_fmaf(w, pv[j][e], acc[e]) : acc[e];
             }
         }
     }
@@ -706,7 +709,7 @@ __global__ void __launch_bounds__(256) k_fa4_combine_few(const FaArgs a) {
     fa4_f4        pv[S];
     float         m[S], l[S];
 #pragma unroll
-    for (int s = 0; s < S; ++s) {  // past the last split: the last one again, weight 0
+    for (int s = 0; s < S; ++s) {  // past the last split: the last one again, never added
         const float * ps = p + (int64_t) (s < last ? s : last) * (D + 4);
         m[s]             = ps[0];
         l[s]             = ps[1];
@@ -726,10 +729,10 @@ __global__ void __launch_bounds__(256) k_fa4_combine_few(const FaArgs a) {
 #pragma unroll
     for (int s = 0; s < S; ++s) {
         const float w = s > last || m[s] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[s] - mm);
-        lt            = w == 0.0f ? lt : __builtin_fmaf(w, l[s], lt);
+        lt            = s <= last ? __builtin_fmaf(w, l[s], lt) : lt;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            t[e] = w == 0.0f ? t[e] : __builtin_fmaf(w, pv[s][e], t[e]);
+            t[e] = s <= last ? __builtin_fmaf(w, pv[s][e], t[e]) : t[e];
         }
     }
     t *= 1.0f / lt;  // no live key: 0 * inf
