@@ -314,7 +314,7 @@ __global__ void __launch_bounds__(256) k_row_q4(const RowCopy K, const RowCopy V
     char *         drow;
     bool           bad;
     uint32_t       bi;
-    if (R.kv && nr * nbpr == 32 && R.ne2 % nr == 0 && t0 + 32 <= total) {
+    if (MI_KV_HEAD_MAJOR && R.kv && nr * nbpr == 32 && R.ne2 % nr == 0 && t0 + 32 <= total) {
         uint32_t i1, i2, i3;
         kv_index(R, dnbpr.div(t0), i1, i2, i3);  // all scalar
         const uint32_t q    = dnbpr.div(j);
