@@ -1375,7 +1375,8 @@ static int lora_desc(const mi_tensor * x, const mi_tensor * a, const mi_tensor *
         return MI_ERR_SHAPE;
     }
     const int64_t m = nrows(*x), n = b->ne[1];
-    if (r > 256 || m > (1 << 30) || (m + 15) / 16 * ((n + 63) / 64) >= kMaxRows || (n + 63) / 64 > 65535) {
+    // a launch's threads are counted in 32 bits: 256 for each 16 rows
+    if (r > 256 || (m + 15) / 16 >= (int64_t) 1 << 24 || (m + 15) / 16 * ((n + 63) / 64) >= kMaxRows || (n + 63) / 64 > 65535) {
         return MI_ERR_UNSUPPORTED;
     }
     l      = LoraArgs{};

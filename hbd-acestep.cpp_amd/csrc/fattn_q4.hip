@@ -1280,16 +1280,32 @@ k_fa4_pre(const FaArgs a) {
 
 constexpr int FA4_W        = 4;   // waves per workgroup of the kernel for few rows
 
-// rows of a workgroup of the kernel for many rows
-static int fa4_bq(int D, bool f32) {
+// rows and threads of a workgroup of the kernel for many rows
+struct Fa4Wg {
+    int rows, threads;
+};
+
+template <int D> static Fa4Wg fa4_wg(bool f32) {
+    return f32 ? Fa4Wg{ Fa4P<D, true>::BQ, 64 * Fa4P<D, true>::W } : Fa4Wg{ Fa4P<D, false>::BQ, 64 * Fa4P<D, false>::W };
+}
+
+static Fa4Wg fa4_wg(int D, bool f32) {
     switch (D) {
         case 64:
-            return f32 ? Fa4P<64, true>::BQ : Fa4P<64, false>::BQ;
+            return fa4_wg<64>(f32);
         case 128:
-            return f32 ? Fa4P<128, true>::BQ : Fa4P<128, false>::BQ;
+            return fa4_wg<128>(f32);
         default:
-            return f32 ? Fa4P<256, true>::BQ : Fa4P<256, false>::BQ;
+            return fa4_wg<256>(f32);
     }
+}
+
+// up to this many splits are merged by a lane for 4 columns of a row, more by a workgroup for a row
+constexpr int FA4_FEW_SPLITS = 8;
+
+// workgroups of 256 threads that the merge of `rows` rows takes
+static int64_t fa4_merge_wgs(int64_t rows, int64_t splits, int D) {
+    return splits <= FA4_FEW_SPLITS ? (rows + 1024 / D - 1) / (1024 / D) : rows;
 }
 
 void flash_attn_q4_plan(FaArgs & a, int D) {
@@ -1308,16 +1324,17 @@ void flash_attn_q4_plan(FaArgs & a, int D) {
     a.mfma              = p.many && a.ngq <= 65535 && (int64_t) a.nb * a.nh <= 65535;
     const int64_t tiles = ((int64_t) a.n_kv + 63) / 64 * (D == 256 ? 2 : 1);
     const int64_t least = a.mfma ? (tiles + FA4_PRE_TILES - 1) / FA4_PRE_TILES : 1;
-    if (a.mfma) {
-        const int bq = fa4_bq(D, a.ty == MI_TYPE_F32);
-        a.rblocks    = (a.rows + bq - 1) / bq;
-    }
-    const int64_t items = (int64_t) a.nb * a.nkv * a.rblocks;
+    const Fa4Wg wg = a.mfma ? fa4_wg(D, a.ty == MI_TYPE_F32) : Fa4Wg{ 16, 64 * FA4_W };
+    a.rblocks      = (a.rows + wg.rows - 1) / wg.rows;
+    const int64_t items = (int64_t) a.nb * a.nkv * a.rblocks, all = (int64_t) a.nb * a.nkv * a.rows;
     int64_t       want  = p.many == (a.mfma != 0) ? p.splits : 1;
     want                = want < FA4_MAX_SPLITS ? want : FA4_MAX_SPLITS;
     a.splits = (int) (want < least ? least : want);
-    if (a.splits > FA4_MAX_SPLITS || items * a.splits >= ((int64_t) 1 << 31) || (int64_t) a.nb * a.nkv * a.rows >= ((int64_t) 1 << 31)) {
-        a.splits = 0;  // more than the merge or a grid takes
+    // more than the merge takes, or than a launch: its threads are counted in 32 bits
+    const int64_t most = ((int64_t) 1 << 32) - 1;
+    if (a.splits > FA4_MAX_SPLITS || items * a.splits > most / wg.threads || all >= ((int64_t) 1 << 31) ||
+        (a.splits > 1 && fa4_merge_wgs(all, a.splits, D) > most / 256)) {
+        a.splits = 0;
     }
 }
 
@@ -1360,18 +1377,17 @@ static void launch_dec(const FaArgs & a, hipStream_t s) {
         MI_LAUNCH((k_fa4_dec<D, OS, 2, FA4_W>), grid, wg, 0, s, a);
     }
     if (a.splits > 1) {
-        const dim3 grid_c((uint32_t) ((int64_t) a.nb * a.nkv * a.rows));
-        const dim3 grid_f((uint32_t) (((int64_t) a.nb * a.nkv * a.rows + 1024 / D - 1) / (1024 / D)));
+        const dim3 grid_m((uint32_t) fa4_merge_wgs((int64_t) a.nb * a.nkv * a.rows, a.splits, D));
         if (a.splits <= 2) {
-            MI_LAUNCH((k_fa4_combine_few<D, 2>), grid_f, dim3(256), 0, s, a);
+            MI_LAUNCH((k_fa4_combine_few<D, 2>), grid_m, dim3(256), 0, s, a);
         } else if (a.splits <= 4) {
-            MI_LAUNCH((k_fa4_combine_few<D, 4>), grid_f, dim3(256), 0, s, a);
-        } else if (a.splits <= 8) {
-            MI_LAUNCH((k_fa4_combine_few<D, 8>), grid_f, dim3(256), 0, s, a);
+            MI_LAUNCH((k_fa4_combine_few<D, 4>), grid_m, dim3(256), 0, s, a);
+        } else if (a.splits <= FA4_FEW_SPLITS) {
+            MI_LAUNCH((k_fa4_combine_few<D, FA4_FEW_SPLITS>), grid_m, dim3(256), 0, s, a);
         } else if (a.splits <= 2 * 1024 / D) {
-            MI_LAUNCH((k_fa4_combine<D, 2>), grid_c, dim3(256), 0, s, a);
+            MI_LAUNCH((k_fa4_combine<D, 2>), grid_m, dim3(256), 0, s, a);
         } else {
-            MI_LAUNCH((k_fa4_combine<D, 8>), grid_c, dim3(256), 0, s, a);
+            MI_LAUNCH((k_fa4_combine<D, 8>), grid_m, dim3(256), 0, s, a);
         }
     }
 }

@@ -267,7 +267,8 @@ int mi_timestep_embedding(const mi_tensor * t, int dim, int max_period, const mi
  * none of the rows a workgroup shares attends to (16 to 256 rows of a KV head; all of
  * one position's with n_q = 1) counts as zeros whatever its bytes are; a block with a
  * non-finite scale of a key that one of them attends to may make the others NaN as
- * well. Q4_0 takes n_kv up to 2^27 and key strides below 32 MiB, others return
+ * well. Q4_0 takes n_kv up to 2^27, key strides below 32 MiB and calls whose launches have fewer
+ * than 2^32 threads (with one position, 2^24 sequences times KV heads), others return
  * MI_ERR_UNSUPPORTED. With BF16 y many rows of q read K rounded to fp16 (2^-11).
  * workspace: device memory of at least mi_flash_attn_ext_workspace() bytes
  * (for the partial results of a split key range; NULL when that is 0). The
@@ -406,7 +407,8 @@ int mi_mul_mat_q8_0_adaln(const void * w, int64_t k, int64_t n, const mi_tensor 
  *   ids:   I32 [m]; a negative id is a row without an adapter, y = y0; an id past the
  *          last adapter is taken as one and counted in *d_err when d_err != NULL
  *   scales: F32 [n_adapters] or NULL (1)
- * Rows of A and B may lie at any element; m up to 2^30.
+ * Rows of A and B may lie at any element; m up to 2^28 - 16, n up to 64 * 65535 with fewer than
+ * 2^31 tiles of 16 rows and 64 columns (others return MI_ERR_UNSUPPORTED).
  * Products and sums keep fp32 accuracy (x and A x as three bf16 parts each on the
  * matrix cores). workspace: device memory of at least mi_lora_add_workspace() bytes,
  * 16-byte aligned; calls that share one race. The size depends on the shapes and on
