@@ -452,6 +452,9 @@ template <int WT> static void launch_w(const LoraArgs & a, hipStream_t s) {
     } else {
         launch_down<WT, 4>(a, s);
     }
+    if (!dry_run() && hipPeekAtLastError() != hipSuccess) {
+        return;  // y, which may be y0, stays as it is: there is no A x to add
+    }
     switch ((a.r + 31) / 32) {
         case 1: launch_up<WT, 1>(a, s); break;
         case 2: launch_up<WT, 2>(a, s); break;
