@@ -1351,11 +1351,22 @@ static void view_span(const mi_tensor & t, uintptr_t & lo, uintptr_t & hi) {
     }
 }
 
+// whether two views of uniformly strided rows share a byte. Rows at one distance (column ranges of a
+// wider buffer) are compared within it; at two distances, the ranges of bytes as a whole.
 static bool views_overlap(const mi_tensor & a, const mi_tensor & b) {
     uintptr_t a0, a1, b0, b1;
     view_span(a, a0, a1);
     view_span(b, b0, b1);
-    return a0 < b1 && b0 < a1;
+    if (!(a0 < b1 && b0 < a1)) {
+        return false;
+    }
+    const uint64_t p = a.nb[1];
+    if (nrows(a) > 1 && nrows(b) > 1 && p == b.nb[1] && p > 0) {
+        const uint64_t wa = (uint64_t) a.ne[0] * type_size(a.type), wb = (uint64_t) b.ne[0] * type_size(b.type);
+        const uint64_t at = b0 >= a0 ? (b0 - a0) % p : (p - (a0 - b0) % p) % p;  // of b's row in a's period
+        return !(wa <= at && wb <= p - at);
+    }
+    return true;
 }
 
 static bool same_view(const mi_tensor & a, const mi_tensor & b) {
