@@ -110,7 +110,9 @@ def _p(t):
     if t is None:
         return None
     c = t.__class__
-    x = t if c is DTensor else t.data
+    x = t if c is DTensor else t.data if isinstance(t, (Q8, Q4)) else None
+    if x.__class__ is not DTensor:  # a class of the caller's: nothing is kept with it
+        return ctypes.byref(desc(t))
     b = x.buf
     k = x.__dict__.get("_arg")
     if k is not None and k[0] is x.shape and k[1] is x.strides and k[2] == x.offset and k[3] == x.dtype and k[4] is b \
