@@ -105,8 +105,8 @@ def desc(t) -> MiTensor:
 
 def _p(t):
     """desc(t) as a call's argument. It stays with the view and is used again as long as the view's fields
-    and its buffer's address are the ones that it was made from: 0.8 us an operand where making it
-    anew takes 2.4 (a decode step's small calls wait for the host)."""
+    and its buffer's address and size (the buffer itself is not kept) are the ones that it was made from:
+    0.8 us an operand where making it anew takes 2.4 (a decode step's small calls wait for the host)."""
     if t is None:
         return None
     c = t.__class__
@@ -115,11 +115,12 @@ def _p(t):
         return ctypes.byref(desc(t))
     b = x.buf
     k = x.__dict__.get("_arg")
-    if k is not None and k[0] is x.shape and k[1] is x.strides and k[2] == x.offset and k[3] == x.dtype and k[4] is b \
-            and k[5] == b.ptr and k[6] is c:
+    if k is not None and k[0] is x.shape and k[1] is x.strides and k[2] == x.offset and k[3] == x.dtype \
+            and k[4] == b.ptr and k[5] == b.nbytes and k[6] is c:
         return k[7]
     p = ctypes.byref(desc(t))
-    x._arg = (x.shape, x.strides, x.offset, x.dtype, b, b.ptr, c, p)
+    if x.shape.__class__ is tuple and x.strides.__class__ is tuple:  # what cannot change in place
+        x._arg = (x.shape, x.strides, x.offset, x.dtype, b.ptr, b.nbytes, c, p)
     return p
 
 
