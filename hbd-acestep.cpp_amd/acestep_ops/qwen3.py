@@ -189,10 +189,11 @@ class Qwen3Layer:
         st = self.stream
         assert S == inp["S"] and N == inp["pos0"].shape[0]
         s0, kv_len, pos, pos0, sets, mask = inp["s0"], inp["kv_len"], inp["pos"], inp["pos0"], inp["sets"], inp["mask"]
+        ids = inp.get("adapter_ids")  # inputs that name no adapters need not say so
         T = N * S
         h2 = hidden.view(T, H)
         qkv_dim = (Nh + 2 * Nkv) * D
-        qkv = self._qkv(h2, qkv_dim, inp["adapter_ids"])
+        qkv = self._qkv(h2, qkv_dim, ids)
         q = qkv[:, 0:Nh * D].unflatten(1, (Nh, D))
         k = qkv[:, Nh * D:(Nh + Nkv) * D].unflatten(1, (Nkv, D))
         v = qkv[:, (Nh + Nkv) * D:qkv_dim].unflatten(1, (Nkv, D))
@@ -207,7 +208,7 @@ class Qwen3Layer:
         attn = self._buf("attn", (N, S, Nh, D))
         ws = self._fa_ws(qf, kv, vv)
         ops.flash_attn_ext(qf, kv, vv, mask, 1.0 / math.sqrt(D), out=attn, workspace=ws, stream=st)
-        y = self._tail(h2, attn.view(T, Nh * D), None if out is None else out.view(T, H), inp["adapter_ids"])
+        y = self._tail(h2, attn.view(T, Nh * D), None if out is None else out.view(T, H), ids)
         return y.view(N, S, H)
 
     def _adapted(self, name, ids):
