@@ -81,7 +81,17 @@ class Qwen3Layer:
                  rope_theta: float = 1e6, clamp_fp16: bool = False, stream=None, adapters=None, adapter_scales=None):
         """w_*: Q8 weights in the GGUF layout (repacked here once); norms: F32 DTensors.
         adapters: {"qkv" | "o" | "gu" | "down": (A (n, r, k), B (n, n_out, r))} bf16 or f16, with
-        adapter_scales F32 (n,) or None (1)."""
+        adapter_scales F32 (n,) or None (1); n is one for all of them, so that an id means the same
+        adapter in every product."""
+        self.adapters, self.adapter_scales = dict(adapters or {}), adapter_scales
+        if not set(self.adapters) <= {"qkv", "o", "gu", "down"}:
+            raise ValueError("adapters: qkv, o, gu, down")
+        counts = {t.shape[0] for ab in self.adapters.values() for t in ab}
+        if self.adapters and adapter_scales is not None:
+            counts.add(adapter_scales.shape[0])
+        if len(counts) > 1:
+            raise ValueError(f"adapters: as many A, B and scales in every product, not {sorted(counts)}")
+        self.n_adapters = counts.pop() if counts else 0
         self.H, self.Nh, self.Nkv, self.D, self.I = H, Nh, Nkv, D, I
         self.eps, self.theta, self.stream = eps, rope_theta, stream
         self.clamp_fp16 = bool(clamp_fp16)
@@ -89,9 +99,6 @@ class Qwen3Layer:
                   for name, w in (("qkv", w_qkv), ("o", w_o), ("gu", w_gate_up), ("down", w_down))}
         self.in_norm_w, self.post_norm_w = in_norm_w, post_norm_w
         self.q_norm_w, self.k_norm_w = q_norm_w, k_norm_w
-        self.adapters, self.adapter_scales = dict(adapters or {}), adapter_scales
-        if not set(self.adapters) <= set(self.w):
-            raise ValueError("adapters: qkv, o, gu, down")
         self.kv_type = kv_type
         if kv_type in ("q8_0", "q4_0"):
             wrap, nb = (ops.Q8, 34) if kv_type == "q8_0" else (ops.Q4, 18)
@@ -127,13 +134,15 @@ class Qwen3Layer:
             return type(c)(c.data[s0:s0 + n, :, :read_len])
         return c[s0:s0 + n, :, :read_len]
 
-    def forward(self, hidden, pos, sets, s0: int, read_len: int, mask, out=None, adapter_ids=None):
+    def forward(self, hidden, pos, sets, s0: int, read_len: int, mask, out=None, adapter_ids=None, err=None):
         """hidden (N, H) F32 -> new hidden (N, H); pos, sets: (N,) I32 device tensors, as
-        adapter_ids, each row's adapter (negative: none)."""
+        adapter_ids, each row's adapter (negative: none). err: I32 device tensor (1,) to which the
+        step adds what it had to leave out: K and V rows without a slot or set, and, once for each
+        product with adapters, rows whose id is past the last adapter."""
         N, Nh, Nkv, D = hidden.shape[0], self.Nh, self.Nkv, self.D
         st = self.stream
         qkv_dim = (Nh + 2 * Nkv) * D
-        qkv = self._qkv(hidden, qkv_dim, adapter_ids)
+        qkv = self._qkv(hidden, qkv_dim, adapter_ids, err)
         q = qkv[:, 0:Nh * D].unflatten(1, (Nh, D))
         k = qkv[:, Nh * D:(Nh + Nkv) * D].unflatten(1, (Nkv, D))
         v = qkv[:, (Nh + Nkv) * D:qkv_dim].unflatten(1, (Nkv, D))
@@ -141,24 +150,24 @@ class Qwen3Layer:
         # new tokens' slots are their positions)
         qo = ops.qk_norm_rope_kv_store(q, self.q_norm_w, k, self.k_norm_w, v, pos, self.eps, D, self.theta,
                                        self.k_cache, self.v_cache, pos, sets=sets, clamp_v=self.clamp_fp16,
-                                       q_out=self._buf("qo", (N, Nh, D)), stream=st)
+                                       q_out=self._buf("qo", (N, Nh, D)), err=err, stream=st)
         kv = self._cache_view(self.k_cache, s0, N, read_len)
         vv = self._cache_view(self.v_cache, s0, N, read_len)
         qf = qo.unflatten(1, (Nh, 1))
         attn = self._buf("attn", (N, 1, Nh, D))
         ws = self._fa_ws(qf, kv, vv)
         ops.flash_attn_ext(qf, kv, vv, mask, 1.0 / math.sqrt(D), out=attn, workspace=ws, stream=st)
-        return self._tail(hidden, attn.view(N, Nh * D), out, adapter_ids)
+        return self._tail(hidden, attn.view(N, Nh * D), out, adapter_ids, err)
 
-    def prefill(self, hidden, kv_pos, s0: int, out=None, adapter_ids=None):
+    def prefill(self, hidden, kv_pos, s0: int, out=None, adapter_ids=None, err=None):
         """hidden (N, S, H) F32 -> new hidden (N, S, H): S new tokens of each of N
         sequences; kv_pos (host ints, N): the slot of each sequence's first new
         token (its earlier tokens already in the cache); sequence b uses set s0 + b
-        and the adapter adapter_ids[b] (host ints, negative: none). prefill_inputs
-        then prefill_run."""
+        and the adapter adapter_ids[b] (host ints, negative: none); err as in forward.
+        prefill_inputs then prefill_run."""
         inp = self.prefill_inputs(kv_pos, hidden.shape[1], s0, adapter_ids)
         self._inputs = inp  # alive until the next call: the launches read them
-        return self.prefill_run(hidden, inp, out)
+        return self.prefill_run(hidden, inp, out, err)
 
     def prefill_inputs(self, kv_pos, S: int, s0: int, adapter_ids=None) -> dict:
         """The host-built inputs of a prefill step, uploaded (qwen3-lm.h:513-533):
@@ -171,17 +180,19 @@ class Qwen3Layer:
         if kv_pos.min() < 0 or kv_len > max_seq:
             raise ValueError(f"prefill: slots [kv_pos, kv_pos + {S}) must lie in [0, {max_seq})")
         if adapter_ids is not None:
-            ids = np.asarray(adapter_ids, np.int32).reshape(-1)
+            ids = np.asarray(adapter_ids, np.int64).reshape(-1)
             if len(ids) != N:
                 raise ValueError("prefill: one adapter id per sequence")
-            adapter_ids = DTensor.from_numpy(np.repeat(ids, S))
+            if self.adapters and ids.max(initial=-1) >= self.n_adapters:
+                raise ValueError(f"prefill: adapter ids below {self.n_adapters}")
+            adapter_ids = DTensor.from_numpy(np.repeat(np.maximum(ids, -1).astype(np.int32), S))
         return {"S": S, "s0": s0, "kv_len": kv_len, "adapter_ids": adapter_ids,
                 "pos": DTensor.from_numpy((kv_pos[:, None] + np.arange(S)[None, :]).astype(np.int32).reshape(N * S)),
                 "pos0": DTensor.from_numpy(kv_pos.astype(np.int32)),
                 "sets": DTensor.from_numpy(np.arange(s0, s0 + N, dtype=np.int32)),
                 "mask": causal_mask(kv_pos, S, kv_len)}
 
-    def prefill_run(self, hidden, inp: dict, out=None):
+    def prefill_run(self, hidden, inp: dict, out=None, err=None):
         """The launches of a prefill step (no host transfer: a graph may capture
         them) on hidden (N, S, H) with inputs from prefill_inputs."""
         N, S, H = hidden.shape
@@ -193,7 +204,7 @@ class Qwen3Layer:
         T = N * S
         h2 = hidden.view(T, H)
         qkv_dim = (Nh + 2 * Nkv) * D
-        qkv = self._qkv(h2, qkv_dim, ids)
+        qkv = self._qkv(h2, qkv_dim, ids, err)
         q = qkv[:, 0:Nh * D].unflatten(1, (Nh, D))
         k = qkv[:, Nh * D:(Nh + Nkv) * D].unflatten(1, (Nkv, D))
         v = qkv[:, (Nh + Nkv) * D:qkv_dim].unflatten(1, (Nkv, D))
@@ -201,55 +212,55 @@ class Qwen3Layer:
         # launch (token t of the flat order is token t % S of sequence t / S)
         qo = ops.qk_norm_rope_kv_store(q, self.q_norm_w, k, self.k_norm_w, v, pos, self.eps, D, self.theta,
                                        self.k_cache, self.v_cache, pos0, sets=sets, clamp_v=self.clamp_fp16,
-                                       q_out=self._buf("qo", (T, Nh, D)), stream=st)
+                                       q_out=self._buf("qo", (T, Nh, D)), err=err, stream=st)
         kv = self._cache_view(self.k_cache, s0, N, kv_len)
         vv = self._cache_view(self.v_cache, s0, N, kv_len)
         qf = qo.view(N, S, Nh, D).permute(0, 2, 1, 3)  # (N, Nh, S, D), ggml's permute(q, 0, 2, 1, 3)
         attn = self._buf("attn", (N, S, Nh, D))
         ws = self._fa_ws(qf, kv, vv)
         ops.flash_attn_ext(qf, kv, vv, mask, 1.0 / math.sqrt(D), out=attn, workspace=ws, stream=st)
-        y = self._tail(h2, attn.view(T, Nh * D), None if out is None else out.view(T, H), ids)
+        y = self._tail(h2, attn.view(T, Nh * D), None if out is None else out.view(T, H), ids, err)
         return y.view(N, S, H)
 
     def _adapted(self, name, ids):
         return ids is not None and name in self.adapters
 
-    def _lora(self, name, y, x, ids):
+    def _lora(self, name, y, x, ids, err):
         """The rows' low-rank updates of product `name`, added to y in place."""
         if self._adapted(name, ids):
             a, b = self.adapters[name]
             ws = self._work("ws_lora_" + name, ops.lora_add_workspace(x, a, b))
-            ops.lora_add(y, x, a, b, ids, self.adapter_scales, out=y, workspace=ws, stream=self.stream)
+            ops.lora_add(y, x, a, b, ids, self.adapter_scales, out=y, workspace=ws, err=err, stream=self.stream)
         return y
 
-    def _qkv(self, hidden, qkv_dim, ids):
+    def _qkv(self, hidden, qkv_dim, ids, err):
         """The input norm and the QKV product of rows of hidden."""
         N, st = hidden.shape[0], self.stream
         if self._adapted("qkv", ids):
             n1 = ops.rms_norm(hidden, self.eps, w=self.in_norm_w, out=self._buf("n1", (N, self.H)), stream=st)
             qkv = ops.mul_mat_q8_0(self.w["qkv"], n1, out=self._buf("qkv", (N, qkv_dim)),
                                    workspace=self._ws("qkv", n1), stream=st)
-            return self._lora("qkv", qkv, n1, ids)
+            return self._lora("qkv", qkv, n1, ids, err)
         # the norm and the product in one call: the normalized rows are made inside
         # the quantization of the product's x
         return ops.mul_mat_q8_0_rms_norm(self.w["qkv"], hidden, self.in_norm_w, self.eps,
                                          out=self._buf("qkv", (N, qkv_dim)), workspace=self._ws("qkv", hidden),
                                          stream=st)
 
-    def _tail(self, hidden, a2, out, ids):
+    def _tail(self, hidden, a2, out, ids, err):
         """The O product, the residual sums, the post-attention norm and the MLP on
         rows of hidden (rows, H) and attention output a2 (rows, Nh * D)."""
         N, H, I = hidden.shape[0], self.H, self.I
         st = self.stream
         ao = ops.mul_mat_q8_0(self.w["o"], a2, out=self._buf("ao", (N, H)), workspace=self._ws("o", a2), stream=st)
-        self._lora("o", ao, a2, ids)
+        self._lora("o", ao, a2, ids, err)
         clamp = (-FP16_MAX, FP16_MAX) if self.clamp_fp16 else None
         if self.clamp_fp16 or self._adapted("gu", ids):
             h1, n2 = ops.add_rms_norm(hidden, ao, self.eps, w=self.post_norm_w, clamp=clamp,
                                       out_sum=self._buf("h1", (N, H)), out_norm=self._buf("n2", (N, H)), stream=st)
             gu = ops.mul_mat_q8_0(self.w["gu"], n2, out=self._buf("gu", (N, 2 * I)), workspace=self._ws("gu", n2),
                                   stream=st)
-            self._lora("gu", gu, n2, ids)
+            self._lora("gu", gu, n2, ids, err)
         else:
             # the residual add, the post-attention norm and the gate/up product in one call
             h1, gu = ops.mul_mat_q8_0_add_rms_norm(self.w["gu"], hidden, ao, self.post_norm_w, self.eps,
@@ -260,7 +271,7 @@ class Qwen3Layer:
             ff = ops.swiglu(gu, out=self._buf("ff", (N, I)), stream=st)
             dn = ops.mul_mat_q8_0(self.w["down"], ff, out=self._buf("dn", (N, H)), workspace=self._ws("down", ff),
                                   stream=st)
-            self._lora("down", dn, ff, ids)
+            self._lora("down", dn, ff, ids, err)
             return (ops.add_clamp if self.clamp_fp16 else ops.add)(h1, dn, out=y, stream=st)
         # swiglu, the down projection and the residual add in one call: the SwiGLU
         # values are made inside the quantization of the product's x, and h1 is
