@@ -11,6 +11,9 @@
 // x, h and y are fp32. Their factors of the products are held as three bf16 parts (24 bits),
 // BF16 weights as they are, F16 weights as two exact bf16 parts: three or five products keep
 // everything but 2^-24 of each term, at matrix-core rates that stay far above what the loads need.
+// The parts of an infinity, and of an x that rounds past bf16's largest, multiply to NaN. So where a
+// product's result is not finite the wave repeats it in fp32 (v_mfma_f32_16x16x4_f32) and takes those
+// elements from there: they are what fp32 operations give, and every other element keeps its bits.
 #include "launch.h"
 #include "rules.h"
 
@@ -37,6 +40,36 @@ __device__ __forceinline__ LrSplit lr_split(const float * x) {
         s.p[2][e]      = (__bf16) (r - (float) b);
     }
     return s;
+}
+
+// whether some lane of the wave has a value that is not finite in c
+template <typename V> __device__ __forceinline__ bool lr_bad(const V * c, int n) {
+    constexpr int E = sizeof(V) / 4;
+    float         t[4] = {};
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            t[(i * E + e) % 4] = __builtin_fmaf(c[i][e], 0.0f, t[(i * E + e) % 4]);
+        }
+    }
+    const float z = (t[0] + t[1]) + (t[2] + t[3]);  // 0 or NaN
+    return __builtin_expect(__builtin_amdgcn_ballot_w64(z != z) != 0, false);
+}
+
+// v, for the compiler another value: what is derived from it is not kept from before
+__device__ __forceinline__ int lr_again(int v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
+// the product of 8 elements of x a lane with 8 weights, in fp32
+__device__ __forceinline__ lr_f4 lr_mul32(const float * x, const float * w, lr_f4 c) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], w[e], c, 0, 0, 0);
+    }
+    return c;
 }
 
 // 8 weights as one or two bf16 parts
@@ -90,9 +123,11 @@ __device__ __forceinline__ int32_t lr_id(const LoraArgs & a, uint32_t t) {
 // rows the chain of ids, weights, products and the sum in LDS (8 rows at rank 16 3.3 us, 48 rows of 24
 // adapters at rank 64 from 4096 keys 7.4 us). A workgroup: 16 rows of x (blockIdx.x), one of a.ks shares of the keys (y), rank
 // block of 16 NR and every a.slots-th distinct adapter of the tile (z). Its 4 waves take
-// alternate steps of 32 keys and are summed in LDS.
+// alternate steps of 32 keys and are summed in LDS. Five waves a SIMD for 4 rank blocks: left to itself the
+// kernel takes registers for its fp32 repeat and runs four (4000 x 2560 at rank 64, 8 adapters in turn, both
+// products 271 us instead of 236).
 template <int WT, int NR>
-__global__ void __launch_bounds__(256) k_lora_down(const LoraArgs a) {
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NR == 4 ? 5 : 1))) k_lora_down(const LoraArgs a) {
     __shared__ lr_f4 part[3][NR][64];
     const int      lane = threadIdx.x & 63, c16 = lane & 15, q4 = lane >> 4;
     const int      wv   = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -139,6 +174,32 @@ __global__ void __launch_bounds__(256) k_lora_down(const LoraArgs a) {
                 c[i] = w[i].mul(xs, c[i]);
             }
         }
+        if (lr_bad(c, NR)) {
+            const int      l  = lr_again(lane);  // addresses made anew: no register holds them across the loop above
+            const uint32_t tt = t0 + (l & 15) < a.m ? t0 + (l & 15) : a.m - 1;
+            const char *   xb = a.x + (int64_t) tt * a.x1 + (l >> 4) * 32;
+#pragma unroll
+            for (int i = 0; i < NR; ++i) {
+                const uint32_t r  = (rb * NR + i) * 16 + (l & 15);
+                const char *   wb = a.a + (int64_t) cur * a.a2 + (int64_t) (r < a.r ? r : a.r - 1) * a.a1 + (l >> 4) * 16;
+                lr_f4          f  = { 0.0f, 0.0f, 0.0f, 0.0f };
+#pragma unroll 1
+                for (uint32_t s = s0 + wv; s < s1; s += 4) {
+                    const lr_f4a x0 = *(const lr_f4a *) (xb + (int64_t) s * 128);
+                    const lr_f4a x1 = *(const lr_f4a *) (xb + (int64_t) s * 128 + 16);
+                    const float  xv[8] = { x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w };
+                    const lr_u4a v = *(const lr_u4a *) (wb + (int64_t) s * 64);
+                    float        wf[8];
+                    unpack16<WT>(make_uint4(v.x, v.y, v.z, v.w), wf);
+                    f = lr_mul32(xv, wf, f);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    c[i][e] = __builtin_isfinite(c[i][e]) ? c[i][e] : f[e];
+                }
+                __builtin_amdgcn_sched_barrier(0);  // one at a time: few registers
+            }
+        }
         __syncthreads();  // the previous adapter's sums are read
         if (wv > 0) {
 #pragma unroll
@@ -176,8 +237,10 @@ __global__ void __launch_bounds__(256) k_lora_down(const LoraArgs a) {
 // Column c of product i is column NT c + i of the wave's: a lane holds NT consecutive columns of
 // 4 rows, and with NT 4 a load or store of y covers 256 consecutive bytes of a row (products of
 // 16 consecutive columns each: 64, and 167 us instead of 138 for 4005 x 19456 at rank 32).
+// The waves a SIMD are those that the registers of the product alone allow. The check for values that are
+// not finite is one fma an element of y, once for all adapters of a tile (1 % at most; once for each: 6 % with 24).
 template <int WT, int NT, int TT, int RS, int U>
-__global__ void __launch_bounds__(256) k_lora_up(const LoraArgs a) {
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NT == 4 ? 2 : RS == 1 ? 5 : RS == 4 ? 3 : 4))) k_lora_up(const LoraArgs a) {
     static_assert(NT == 1 || NT == 4, "a dword or a float4 of y per lane and row");
     constexpr int RQ = RS * 32 + 8;  // row of h in LDS: 16 rows on distinct banks
     constexpr int R  = 16 * TT;
@@ -268,7 +331,8 @@ __global__ void __launch_bounds__(256) k_lora_up(const LoraArgs a) {
         for (int g = 0; g < G; ++g) {
             const int    i = i0 + 256 * g, t = i / (RS * 32), r = i - t * RS * 32;
             const float  x = on[g] ? v[g] * sc[g] : 0.0f;
-            const __bf16 x0 = (__bf16) x;
+            // a finite x stays finite in its first part: no larger than bf16's largest
+            const __bf16 x0 = (__bf16) (__builtin_isfinite(x) ? __builtin_amdgcn_fmed3f(x, -0x1.fep127f, 0x1.fep127f) : x);
             const float  r0 = x - (float) x0;
             const __bf16 x1 = (__bf16) r0;
             hs[t * RQ + r]           = x0;
@@ -278,6 +342,60 @@ __global__ void __launch_bounds__(256) k_lora_up(const LoraArgs a) {
     }
     __syncthreads();
     const bool vec = a.r % 8 == 0;
+    // 8 ranks from 32 s + 8 q4 on of a column of B; past the rank: zeros
+    auto weights = [&](const char * p, int s) -> uint4 {
+        const int r0 = s * 32 + 8 * q4;
+        uint4     v  = make_uint4(0, 0, 0, 0);
+        if (r0 + 8 <= (int) a.r) {
+            const lr_u4a x = *(const lr_u4a *) (p + s * 64);
+            v              = make_uint4(x.x, x.y, x.z, x.w);
+        } else if (!vec && r0 < (int) a.r) {
+            uint16_t x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                x[e] = r0 + e < (int) a.r ? *(const uint16_t *) (p + s * 64 + e * 2) : 0;
+            }
+            v = make_uint4(x[0] | (uint32_t) x[1] << 16, x[2] | (uint32_t) x[3] << 16, x[4] | (uint32_t) x[5] << 16,
+                           x[6] | (uint32_t) x[7] << 16);
+        }
+        return v;
+    };
+    // The elements of y named in `left` (bit (tt * 4 + e) NT + i), which hold y0: the product in fp32 is added.
+    auto repeat = [&](uint32_t nb, uint32_t left) {
+        uint64_t todo = rows;
+        while (todo) {
+            const int32_t cur = __builtin_amdgcn_readlane(idl, __builtin_ctzll(todo));
+            todo &= ~__builtin_amdgcn_ballot_w64(idl == cur);
+#pragma unroll 1
+            for (int ti = 0; ti < TT * NT; ++ti) {
+                const int      l = lr_again(lane), tt = ti / NT, i = ti - tt * NT;
+                const uint32_t n = nb + NT * (l & 15) + i < a.n ? nb + NT * (l & 15) + i : a.n - 1;
+                const char *   p = a.b + (int64_t) cur * a.b2 + (l >> 4) * 16 + (int64_t) n * a.b1;
+                lr_f4          f = { 0.0f, 0.0f, 0.0f, 0.0f };
+#pragma unroll 1
+                for (int s = 0; s < RS; ++s) {
+                    const __bf16 * hp = hs + (tt * 16 + (l & 15)) * RQ + s * 32 + 8 * (l >> 4);
+                    float          h[8], w[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {  // an infinity's other parts are NaN
+                        const float h0 = (float) hp[e], h1 = (float) hp[R * RQ + e] + (float) hp[2 * R * RQ + e];
+                        h[e]           = __builtin_isinf(h0) ? h0 : h0 + h1;
+                    }
+                    unpack16<WT>(weights(p, s), w);
+                    f = lr_mul32(h, w, f);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int     r  = tt * 16 + 4 * (l >> 4) + e;
+                    const int32_t it = __shfl(idl, r, 64);
+                    if (it == cur && left >> ((tt * 4 + e) * NT + i) & 1) {
+                        float * yp = (float *) (a.y + (int64_t) (t0 + r) * a.y1 + (int64_t) n * 4);
+                        *yp        = *yp + f[e];
+                    }
+                }
+            }
+        }
+    };
     for (; n0 < a.n; n0 += gridDim.y * (64 * NT)) {
 #pragma unroll
         for (int tt = 0; tt < TT; ++tt) {
@@ -304,21 +422,7 @@ __global__ void __launch_bounds__(256) k_lora_up(const LoraArgs a) {
                         const char *   p = bp + (int64_t) (n < a.n ? n : a.n - 1) * a.b1;
 #pragma unroll
                         for (int s = 0; s < RS; ++s) {
-                            const int r0 = s * 32 + 8 * q4;
-                            uint4     v  = make_uint4(0, 0, 0, 0);
-                            if (r0 + 8 <= (int) a.r) {
-                                const lr_u4a x = *(const lr_u4a *) (p + s * 64);
-                                v              = make_uint4(x.x, x.y, x.z, x.w);
-                            } else if (!vec && r0 < (int) a.r) {
-                                uint16_t x[8];
-#pragma unroll
-                                for (int e = 0; e < 8; ++e) {
-                                    x[e] = r0 + e < (int) a.r ? *(const uint16_t *) (p + s * 64 + e * 2) : 0;
-                                }
-                                v = make_uint4(x[0] | (uint32_t) x[1] << 16, x[2] | (uint32_t) x[3] << 16,
-                                               x[4] | (uint32_t) x[5] << 16, x[6] | (uint32_t) x[7] << 16);
-                            }
-                            w[u][s][i].raw = v;
+                            w[u][s][i].raw = weights(p, s);
                         }
                     }
                 }
@@ -362,16 +466,41 @@ __global__ void __launch_bounds__(256) k_lora_up(const LoraArgs a) {
             }
         }
         const uint32_t n = n0 + NT * c16;
-        if (n + NT <= a.n) {
+        const bool     in  = n + NT <= a.n;
+        const bool     bad = lr_bad(acc[0], TT * 4);
+        uint32_t       left = 0;
+        auto           mine = [&](int tt, int e) { return in && (NT == 1 ? own >> (4 * q4 + e) & 1 : t0 + tt * 16 + 4 * q4 + e < a.m); };
+        if (bad) {
+            const int      l = lr_again(lane);
+            const uint32_t nn = n0 + NT * (l & 15);
 #pragma unroll
             for (int tt = 0; tt < TT; ++tt) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    if (NT == 1 ? own >> (4 * q4 + e) & 1 : t0 + tt * 16 + 4 * q4 + e < a.m) {
-                        *(lr_y *) (a.y + row(tt, e) * a.y1 + (int64_t) n * 4) = acc[tt][e];
+                    const uint32_t t  = t0 + tt * 16 + 4 * (l >> 4) + e;
+                    const lr_y     y0 = *(const lr_y *) (a.y0 + (int64_t) (t < a.m ? t : a.m - 1) * a.y01 + (int64_t) (nn + NT <= a.n ? nn : a.n - NT) * 4);
+#pragma unroll
+                    for (int i = 0; i < NT; ++i) {
+                        if (!__builtin_isfinite(acc[tt][e][i])) {
+                            left |= (mine(tt, e) ? 1u : 0u) << ((tt * 4 + e) * NT + i);
+                            acc[tt][e][i] = y0[i];
+                        }
                     }
+                    __builtin_amdgcn_sched_barrier(0);  // few registers
                 }
             }
+        }
+#pragma unroll
+        for (int tt = 0; tt < TT; ++tt) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (mine(tt, e)) {
+                    *(lr_y *) (a.y + row(tt, e) * a.y1 + (int64_t) n * 4) = acc[tt][e];
+                }
+            }
+        }
+        if (bad) {
+            repeat(n0, left);
         }
     }
 }

@@ -410,7 +410,8 @@ int mi_mul_mat_q8_0_adaln(const void * w, int64_t k, int64_t n, const mi_tensor 
  * Rows of A and B may lie at any element; m up to 2^28 - 16, n up to 64 * 65535 with fewer than
  * 2^31 tiles of 16 rows and 64 columns (others return MI_ERR_UNSUPPORTED).
  * Products and sums keep fp32 accuracy (x and A x as three bf16 parts each on the
- * matrix cores). workspace: device memory of at least mi_lora_add_workspace() bytes,
+ * matrix cores); infinities and NaN come out where fp32 operations bring them, and
+ * change no other element. workspace: device memory of at least mi_lora_add_workspace() bytes,
  * 16-byte aligned; calls that share one race. The size depends on the shapes and on
  * the current device's CU count. */
 int mi_lora_add_workspace(const mi_tensor * x, const mi_tensor * a, const mi_tensor * b, size_t * bytes);
