@@ -554,9 +554,9 @@ template <int WT, int NR> static void launch_down(const LoraArgs & a, hipStream_
 
 template <int WT, int RS> static void launch_up(const LoraArgs & a, hipStream_t s) {
     if (lora_wide(a.m, a.n)) {
-        // rows in tiles of 32 (16 at high ranks), column blocks of 256 over enough workgroups for 6 per CU (both
-        // products, us, for 3 / 4 / 6 / 8 / 12: 4005 x 19456 155.4 / 158.2 / 153.0 / 154.9 / 156.6; 793 x 19456 41.3 / 40.7 /
-        // 41.9 / 43.5 / 43.4; 1500 x 19456 65.2 / 62.2 / 63.0 / 63.1 / 65.4)
+        // rows in tiles of 32 (16 at high ranks), column blocks of 256 over enough workgroups for 6 per CU: within 3 % of
+        // the best at each size (both products, us, for 3 / 4 / 6 / 8 / 12: 4005 x 19456 155.4 / 158.2 / 153.0 / 154.9 / 156.6;
+        // 793 x 19456 41.3 / 40.7 / 41.9 / 43.5 / 43.4; 1500 x 19456 65.2 / 62.2 / 63.0 / 63.1 / 65.4)
         constexpr int  TT    = RS < 8 ? 2 : 1;
         const uint32_t tiles = (a.m + 16 * TT - 1) / (16 * TT), blocks = (a.n + 255) / 256;
         const uint32_t want  = ((uint32_t) num_cus() * 6 + tiles - 1) / tiles;

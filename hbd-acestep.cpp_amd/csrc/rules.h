@@ -79,11 +79,14 @@ inline bool logits_small_tiles(uint32_t rows, int64_t n_vocab, uint32_t cus) {
 
 // Adapters' second product, m rows of n columns: whether a lane takes 4 columns of each of its rows, in
 // tiles of 32 rows (16 at high ranks) and 256 columns, not one column in tiles of 16 rows and 64
-// columns whose adapters are shared out over workgroups. Wide tiles move y at the rate of memory; small
-// ones give every adapter of few rows a workgroup (us wide / narrow, both products: 64 x 6144, 8
-// adapters 16.5 / 11.7; 200 x 6144 19.6 / 16.7; 500 x 6144 30.7 / 34.1; 64 x 19456, one 11.4 / 11.7;
-// 100 x 19456 13.1 / 14.9; 200 x 2560, 24 adapters of rank 64 62.9 / 36.0; 1000 x 1024 11.4 / 11.3; 600 x
-// 2560 12.9 / 14.6; 2000 x 19456, 16 in turn 249 / 291; 1000 x 6144, 24 in turn 82.5 / 73.8).
+// columns whose adapters are shared out over workgroups. Wide tiles move y at the rate of memory, but
+// multiply all their rows by each of their adapters; small ones give every adapter of few rows a
+// workgroup. Which rows share an adapter is device memory, so the rule sees sizes only. us wide / narrow,
+// both products: 64 x 6144, 8 adapters in turn 16.5 / 11.7; 200 x 6144 19.6 / 16.7; 500 x 6144 30.7 / 32.5; 64 x
+// 19456, one 11.4 / 11.7; 100 x 19456 13.1 / 14.9; 200 x 2560, 24 of rank 64 62.4 / 36.5; 1000 x 1024 11.4 / 11.3;
+// 600 x 2560 12.9 / 14.6; 2000 x 19456, 16 249 / 280; 4000 x 2560, 8 of rank 64 236 / 268; 1000 x 6144, 24 in runs of 40
+// 24.3 / 27.8. What it loses: 24 adapters in turn at 300 to 1000 x 6144 and 100 to 200 x 19456, 9 to 16 % (1000 x
+// 6144 82.1 / 70.6), 8 in turn right past the border, 11 % (250 x 6144 19.6 / 17.7).
 inline bool lora_wide(int64_t m, int64_t n) {
     return n >= 4 && m * n >= 1500000;
 }
@@ -127,6 +130,8 @@ struct Fa4Plan {
 //   16 heads on 8: 64 positions on 464 keys 13.3 / 22.8, 12.5 / 18.8; 257 on 387 18.9 / 35.8, 16.8 / 24.2;
 //                  512 on 512 23.5 / 34.8, 20.9 / 26.3; 1024 on 1024 65 / 51, 52 / 37; 2048 on 2048 207 / 98, 146 / 58
 //   32 on 8, 8 sequences: 16 on 4016 59 / 96, 48 / 40; 64 on 4064 194 / 108, 146 / 66; 128 on 128 45 / 28, 35 / 17
+// What it loses where both were timed: 64 values, 32 on 8, 8 sequences, 16 on 4016 in F32 38.2 / 42.4 (many taken); 256
+// values, 16 on 8, 512 on 512 39.5 / 41.2 (many taken); all others go to the quicker side or lie within 5 %.
 inline Fa4Plan fa4_plan(int64_t heads, int64_t rows, int64_t n_kv, int d, bool f32, bool one, int64_t cus) {
     const int64_t all = heads * rows;
     // 16 rows a workgroup
