@@ -91,7 +91,6 @@ class Qwen3Layer:
             counts.add(adapter_scales.shape[0])
         if len(counts) > 1:
             raise ValueError(f"adapters: as many A, B and scales in every product, not {sorted(counts)}")
-        self.n_adapters = counts.pop() if counts else 0
         self.H, self.Nh, self.Nkv, self.D, self.I = H, Nh, Nkv, D, I
         self.eps, self.theta, self.stream = eps, rope_theta, stream
         self.clamp_fp16 = bool(clamp_fp16)
@@ -110,6 +109,11 @@ class Qwen3Layer:
         else:
             raise ValueError("kv_type: q8_0, q4_0 or f16")
         self._bufs, self._outgrown = {}, []
+
+    @property
+    def n_adapters(self) -> int:
+        """The adapters' count, of those that the layer has now: they may be given to it later."""
+        return max((a.shape[0] for a, _ in self.adapters.values()), default=0)
 
     def _buf(self, name, shape, dtype="f32"):
         b = self._bufs.get(name)

@@ -50,3 +50,13 @@ def test_what_a_prompt_leaves_out_is_counted(dev):
     inp["sets"] = to_dev(np.array([c.s0, 77], np.int32))
     c.layer.prefill_run(hidden, inp, err=err)
     assert err.item() == 4 * 5 + 2 * 5 * c.Nkv
+
+
+def test_adapters_given_to_a_layer_later(dev):
+    c, later = Case("small"), Case("small", only=())
+    later.layer.adapters.update(c.layer.adapters)
+    hidden = to_dev(randn((2, 5, c.H), seed=11))
+    got = [to_np(x.layer.prefill(hidden, [3, 0], x.s0, adapter_ids=[1, 3])) for x in (c, later)]
+    assert np.array_equal(*got)
+    with pytest.raises(ValueError):
+        later.layer.prefill(hidden, [3, 0], later.s0, adapter_ids=[1, 4])

@@ -31,6 +31,7 @@ def test_stacks_that_do_not_agree(adapters, scales):
 @pytest.mark.parametrize("ids", [[0, 3], [1 << 32, 0], [0], [0, 1, 2]])
 def test_ids_of_a_prompt(ids):
     layer = Qwen3Layer.__new__(Qwen3Layer)
-    layer.kv_type, layer.k_cache, layer.adapters, layer.n_adapters = "f16", _t(2, 1, 128, 64, dtype="f16"), {"o": None}, 3
+    layer.kv_type, layer.k_cache = "f16", _t(2, 1, 128, 64, dtype="f16")
+    layer.adapters = {"o": (_t(3, 8, 64), _t(3, 64, 8))}
     with pytest.raises(ValueError, match="adapter id"):
         layer.prefill_inputs(np.array([0, 5]), 4, 0, adapter_ids=ids)
