@@ -74,6 +74,12 @@ __device__ __forceinline__ void fa4_block(const Fa4Raw & r, int blk, float & d, 
     d = f16_lo(blk & 1 ? r.w[0] >> 16 : r.w[0]);
 }
 
+// The scale of a block of K whose levels are summed before it is applied: an infinite one becomes NaN, as
+// the block's zeros (level 8) times it are. A sum's sign would make the scores -inf, and leave the key out.
+__device__ __forceinline__ float fa4_scale(float d) {
+    return d + (d - d);
+}
+
 __device__ __forceinline__ uint32_t fa4_bits(fa4_h2 v) {
     return __builtin_bit_cast(uint32_t, v);
 }
@@ -397,7 +403,7 @@ k_fa4_dec(const FaArgs a) {
                 for (int e = 0; e < 4; ++e) {
                     *(uint32_t *) (kp + e * 4 * NB) = q[e];
                 }
-                dkl[blk * F::DS + key] = d;
+                dkl[blk * F::DS + key] = fa4_scale(d);
                 fa4_block(vr[it], blk, d, q);
                 *(uint4 *) (vl + F::voff(key) + blk * 16) = make_uint4(q[0], q[1], q[2], q[3]);
                 d   = live >> key & 1 ? d : 0.0f;
@@ -905,7 +911,7 @@ k_fa4_pre(const FaArgs a) {
             d = live >> key & 1 ? d : 0.0f;
         }
         if (OS && !isv) {
-            dl[blk * F::DS + key] = d;  // fp32: nothing to scale
+            dl[blk * F::DS + key] = fa4_scale(d);  // fp32: nothing to scale
         }
         d *= fl & (isv ? 1u : 2u) ? 0.0625f : 1.0f;
         const _Float16 dh = (_Float16) d;

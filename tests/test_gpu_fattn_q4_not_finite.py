@@ -2,6 +2,7 @@
 are split over: also where that key is the only one its split attends to, or its weight underflows to zero."""
 import numpy as np
 import pytest
+import q4
 from helpers import randn, to_dev, to_np
 from oracle import oracle as orc
 from test_gpu_fattn_q4 import _cache, _mask_dev, _q
@@ -72,3 +73,20 @@ def test_the_only_live_key_of_a_split_many_rows(dev, D, nh, n_q, dt, out):
     assert _splits(qv, kd, vd, summary) >= 2, "the keys are split"
     assert np.isnan(y[:, 256:]).all()
     assert np.isfinite(y[:, :256]).all()
+
+
+@pytest.mark.parametrize("dt,out", [("f32", "f32"), ("bf16", "bf16")])
+@pytest.mark.parametrize("D,N,nh,nkv,n_q,n", [(64, 1, 4, 2, 1, 100), (128, 2, 8, 2, 1, 700), (256, 1, 2, 1, 5, 90), (64, 8, 32, 8, 130, 200),
+                                              (128, 8, 32, 8, 130, 200), (256, 8, 16, 4, 130, 100)])
+def test_an_infinity_in_a_live_key(dev, D, N, nh, nkv, n_q, n, dt, out):
+    """Its block reads back as no finite value, so every row that attends to it is NaN, whatever its sign and q's."""
+    print(f"q4 attention, an infinite K element D={D} n_q={n_q} {dt}->{out}", flush=True)
+    x = randn((N, nkv, n, D), seed=2)
+    x[:, :, 17, 5], x[:, ::2, n - 3, D - 1] = np.inf, -np.inf
+    k, v = q4.quantize(x), _cache(N, nkv, n, D, 3)
+    mask = np.zeros((1, 1, n_q, n))
+    _, _, _, y = _run(D, N, nh, nkv, n_q, dt, out, k, v, mask)
+    assert np.isnan(y).all()
+    mask[..., 17] = mask[..., n - 3] = -np.inf
+    _, _, _, y = _run(D, N, nh, nkv, n_q, dt, out, k, v, mask)
+    assert np.isfinite(y).all()
