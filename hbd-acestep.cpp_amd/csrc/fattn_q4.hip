@@ -11,12 +11,19 @@
 //         of the row's largest; the matrix cores' sums of whole numbers are exact, where
 //         sums of 24-bit terms are cut at each step (measured over the LM's decode size:
 //         y off by 4.1e-6 with two fp16 of any size, 2-norm over 2-norm, torch's fp32 6e-7).
+//         So elements far below their row's largest keep fewer bits than fp32: with one of the
+//         row 10 / 100 / 1000 times the rest, on a channel that K hardly holds, y is off by
+//         3.8e-7 / 1.9e-6 / 2.5e-5 (fp32 scores: 1.1e-7); a third part would be half as many
+//         products again.
 //  levels as fp16 numbers -8 .. 7, by one mask-and-or and one packed add each two (the
 //         nibbles' bits as they are, subnormals n 2^-24, with the -8 in the accumulator's
 //         start, took fewer instructions but 4 registers a block for that start).
 //  P, V   F32 y: P and v = (level - 8) d as a high and a low fp16 each (v exact, P to
-//         22 bits), three products; BF16 y: one fp16 each (2^-11 against y's 2^-8).
-//         d above 8188 would leave fp16: tiles with one scale v by 2^-4, P by 2^4.
+//         22 bits), three products; BF16 y: one fp16 each (2^-11 against y's 2^-8: the error
+//         against 64 bits is 1 to 2 % above that of 32-bit operations rounded to BF16).
+//         d above 8188 would leave fp16: tiles with one scale v by 2^-4, P by 2^4; there
+//         a d below 2^-10 loses bits (held / 16 it leaves fp16's normal numbers: an absolute
+//         2^-21 of d).
 // Sums, maxima and the running output are fp32.
 #include "launch.h"
 #include "rules.h"
@@ -184,7 +191,8 @@ typedef uint32_t fa4_u2h __attribute__((ext_vector_type(2), aligned(2)));  // 4 
 // Bound by a tile's chain and its unpacking: a lone wave takes 1.5 us a tile (D = 128, BF16 y; F32 1.6),
 // three on a SIMD 2.1 for a tile each. Three waves a SIMD (F32 y, a mask row each, left to itself takes 171
 // registers and two waves: 5 positions on 20000 46.4 us instead of 39.0, 16 on 4016 66.4 instead of 55.9), two at
-// D = 256 (one: 7 positions on 30177, BF16 y, 63 us instead of 52; 8 rows on 3001 23.3 instead of 24.0). 2 rows
+// D = 256 (one: 7 positions on 30177, BF16 y, 63 us instead of 52; 8 rows on 3001 23.3 instead of 24.0; F32 y then
+// spills 3, 9 and 21 of 256 registers without a mask, with one mask row, with a row each). 2 rows
 // of 60013 keys, 32 heads on 8, 128, BF16 y: 29 us, 3.7 TB/s; 8 of up to 6600, F32 y: 21 us, 1.8 TB/s.
 // Tiles of 64 keys at D = 128 leave half as many waves a turn; 8 waves a workgroup: 257 positions on
 // 387 keys 25.8 us instead of 19.0, 64 on 2064 29.6 instead of 22.8.
@@ -768,8 +776,8 @@ __global__ void __launch_bounds__(256) k_fa4_combine_few(const FaArgs a) {
 // The maximum that p refers to moves only when a row's grows by more than 2^3, so most tiles
 // need no reduction over lanes; the row sums are products with ones. Masks are looked up per tile in
 // k_fa_mask_summary's bytes.
-// Bound by unpacking and exponentials beside the matrix cores (busy 28 % of the cycles; two waves a
-// SIMD is what the registers leave). 8 x 2048 positions, 32 heads on 8, 128: BF16 y without a mask
+// Bound by unpacking and exponentials beside the matrix cores (busy 33 % of the cycles, vector issue 58 %;
+// two waves a SIMD is what the registers leave). 8 x 2048 positions, 32 heads on 8, 128: BF16 y without a mask
 // 642 us, 856 TFLOP/s, causal 381 and 16 for the summary; F32 y 1292 and 752. 8 waves (256 rows) in BF16:
 // 626 without a mask, but 2048 positions on 6144 keys 239 instead of 229.
 template <int D, bool OS> struct Fa4P {

@@ -269,7 +269,10 @@ int mi_timestep_embedding(const mi_tensor * t, int dim, int max_period, const mi
  * non-finite scale of a key that one of them attends to may make the others NaN as
  * well. Q4_0 takes n_kv up to 2^27, key strides below 32 MiB and calls whose launches have fewer
  * than 2^32 threads (with one position, 2^24 sequences times KV heads), others return
- * MI_ERR_UNSUPPORTED. With BF16 y many rows of q read K rounded to fp16 (2^-11).
+ * MI_ERR_UNSUPPORTED. With BF16 y the probabilities and V are rounded to fp16 (2^-11), and many
+ * rows of q read K rounded to fp16 too; with F32 y the probabilities keep 22 bits. Where a V
+ * block of 32 or 64 neighbouring keys has a scale past 8188, their other V scales are kept to
+ * an absolute 2^-21.
  * workspace: device memory of at least mi_flash_attn_ext_workspace() bytes
  * (for the partial results of a split key range; NULL when that is 0). The
  * size depends on the shapes and on the current device's CU count. */
